@@ -54,7 +54,8 @@ enum frsa_status {
   FRSA_ERR_DEVICE_TIMEOUT = 7,  /* a kernel gave up on a bounded wait (see frsa_query_status) */
   FRSA_ERR_NO_DEVICE = 8,       /* the current device is not sm_100 */
   FRSA_ERR_WORKSPACE = 9,       /* the backward workspace is missing or too small */
-  FRSA_ERR_SCRATCH_LIMIT = 10   /* B*H*N*D exceeds frsa_bwd_noalloc_max_elements() */
+  FRSA_ERR_SCRATCH_LIMIT = 10,  /* B*H*N*D exceeds frsa_bwd_noalloc_max_elements() */
+  FRSA_ERR_BAD_INDEX = 11       /* a kernel met an index outside its tensor (see frsa_query_status) */
 };
 
 typedef struct frsa_attn_args {
@@ -160,7 +161,9 @@ const char* frsa_last_error_detail(void);
 
 /* Synchronizes the current device, returns FRSA_ERR_DEVICE_TIMEOUT if any
  * kernel recorded a bounded-wait timeout since the last call (and clears it),
- * FRSA_ERR_LAUNCH on a sticky CUDA error, else FRSA_OK. */
+ * FRSA_ERR_BAD_INDEX if a serving kernel met a page, a length, a position or a
+ * sequence boundary outside its tensor (and clears it; the access was
+ * skipped), FRSA_ERR_LAUNCH on a sticky CUDA error, else FRSA_OK. */
 int frsa_query_status(void);
 
 /* QKV projection with the 2D RoPE applied in its epilogue: for x [B*N, C]
@@ -236,6 +239,112 @@ typedef struct frsa_convert_args {
 
 int frsa_convert_in(const frsa_convert_args* args, void* stream);
 int frsa_convert_out(const frsa_convert_args* args, void* stream);
+
+/* ---- Serving: a paged key-value cache, and causal attention over prompts.
+ *
+ * No counterpart in the reference, whose attention is unmasked over one fixed
+ * grid of tokens (fa_rope_full .py:91-315).
+ *
+ * Tokens of several sequences are packed: q [T, Hq, D], k and v [T, Hkv, D],
+ * Hkv dividing Hq (query head h reads kv head h / (Hq / Hkv)); sequence b
+ * holds the tokens [cu_seqlens[b], cu_seqlens[b + 1]). A cache is [num_pages,
+ * Hkv, page_size, D]; token i of sequence b lies in page
+ * block_table[b * block_table_stride + i / page_size], slot i % page_size.
+ * Every index array is int32 on the device. Index values outside their range
+ * are not followed: the access is skipped and frsa_query_status reports
+ * FRSA_ERR_BAD_INDEX.
+ *
+ * Element strides (token, head) of q, k, v and (page, head, slot) of both
+ * caches; the d stride is 1. All zero = contiguous. They are positive
+ * multiples of 16 bytes, and the pointers 16-byte aligned. D % 8 == 0,
+ * D <= 128; dtype BF16 or F16. */
+
+/* Append: for token t of sequence b, at index i = start_lens[b] + t -
+ * cu_seqlens[b] (cu_seqlens NULL: one token per sequence, T == B), with
+ * rotation row p = positions[t] (positions NULL: p = i; p = -1: not rotated):
+ * q_out[t] = R_p q[t], k_out[t] = R_p k[t] (rotated in f32, rounded once),
+ * and R_p k[t], v[t] are written to the caches. q_out and k_out are
+ * contiguous; k_out may be NULL. Two tokens must not share a slot. */
+typedef struct frsa_paged_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* block_table;  /* [B, max_pages], row stride block_table_stride */
+  const int32_t* start_lens;   /* [B] tokens cached before the call */
+  const int32_t* cu_seqlens;   /* [B + 1] or NULL */
+  const int32_t* positions;    /* [T] or NULL */
+  const float* cosp;           /* [n_pos, D/2] */
+  const float* sinp;
+  int64_t T, B, Hq, Hkv, D, n_pos;
+  int64_t num_pages, page_size, max_pages, block_table_stride;
+  int64_t q_strides[2];
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t cache_strides[3];
+  int32_t dtype;
+} frsa_paged_append_args;
+
+int frsa_paged_append(const frsa_paged_append_args* args, void* stream);
+
+/* Attention of one token per sequence over the cache:
+ * o[b, h] = sum_j softmax_j(scale q[b, h] . K_j) V_j over the cached tokens
+ * j < seq_lens[b]; q and K arrive rotated. seq_lens[b] = 0: o = 0, lse = -inf.
+ * q [B, Hq, D], o contiguous [B, Hq, D], lse [B, Hq] (natural log) or NULL.
+ *
+ * The work is split over the cache's length and joined inside one launch
+ * through the workspace (frsa_paged_decode_workspace_bytes() bytes, 16-byte
+ * aligned). Zero the workspace before its first use; every call leaves it
+ * ready for the next. Calls that may run at the same time need workspaces of
+ * their own. The result does not depend on timing. */
+typedef struct frsa_paged_decode_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  float* lse;
+  const int32_t* block_table;
+  const int32_t* seq_lens;     /* [B] cached tokens, the new one included */
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, Hq, Hkv, D;
+  int64_t num_pages, page_size, max_pages, block_table_stride;
+  int64_t q_strides[2];        /* (sequence, head) */
+  int64_t cache_strides[3];
+  float scale;
+  int32_t dtype;
+} frsa_paged_decode_args;
+
+int frsa_paged_decode(const frsa_paged_decode_args* args, void* stream);
+
+/* Workspace of frsa_paged_decode on the current device (the same for every
+ * shape). */
+size_t frsa_paged_decode_workspace_bytes(void);
+
+/* Causal attention over whole packed prompts:
+ * o[t, h] = sum_j softmax_j(scale q[t, h] . k[j, h']) v[j, h'] over the
+ * tokens j <= t of t's sequence; q and k arrive rotated. o contiguous
+ * [T, Hq, D], lse [Hq, T] (natural log) or NULL. Tokens from cu_seqlens[B] on
+ * belong to no sequence: o = 0, lse = -inf. Hq / Hkv <= 128. */
+typedef struct frsa_prompt_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  const int32_t* cu_seqlens;   /* [B + 1] */
+  int64_t T, B, Hq, Hkv, D;
+  int64_t q_strides[2];
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  float scale;
+  int32_t dtype;
+} frsa_prompt_args;
+
+int frsa_prompt_fwd(const frsa_prompt_args* args, void* stream);
 
 /* FRSA_ABI_VERSION of the loaded library. */
 int frsa_abi_version(void);

@@ -15,6 +15,11 @@ from .attention import (  # noqa: F401
     fused_rope_attention_bwd,
 )
 from .ops import sdpa_fa_rope_op  # noqa: F401  (registers torch.ops.frsa.*)
+from .serving import (  # noqa: F401
+    paged_decode_attention,
+    paged_rope_append,
+    prompt_attention,
+)
 
 __all__ = [
     "build_axial_rope_pairs",
@@ -25,4 +30,7 @@ __all__ = [
     "fused_rope_attention_fwd",
     "fused_rope_attention_bwd",
     "sdpa_fa_rope_op",
+    "paged_rope_append",
+    "paged_decode_attention",
+    "prompt_attention",
 ]

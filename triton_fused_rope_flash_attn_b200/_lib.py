@@ -29,6 +29,10 @@ EXPORTED_SYMBOLS = (
     "frsa_last_error_detail",
     "frsa_bwd_noalloc",
     "frsa_bwd_noalloc_max_elements",
+    "frsa_paged_append",
+    "frsa_paged_decode",
+    "frsa_paged_decode_workspace_bytes",
+    "frsa_prompt_fwd",
 )
 
 
@@ -130,6 +134,45 @@ class FrsaConvertArgs(ctypes.Structure):
     ]
 
 
+class FrsaPagedAppendArgs(ctypes.Structure):
+    """Mirror of ``frsa_paged_append_args`` (include/frsa.h)."""
+
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in (
+            "q", "k", "v", "q_out", "k_out", "k_cache", "v_cache", "block_table", "start_lens",
+            "cu_seqlens", "positions", "cosp", "sinp")]
+        + [(n, ctypes.c_int64) for n in (
+            "T", "B", "Hq", "Hkv", "D", "n_pos", "num_pages", "page_size", "max_pages",
+            "block_table_stride")]
+        + [("q_strides", ctypes.c_int64 * 2), ("k_strides", ctypes.c_int64 * 2),
+           ("v_strides", ctypes.c_int64 * 2), ("cache_strides", ctypes.c_int64 * 3),
+           ("dtype", ctypes.c_int32)])
+
+
+class FrsaPagedDecodeArgs(ctypes.Structure):
+    """Mirror of ``frsa_paged_decode_args`` (include/frsa.h)."""
+
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in (
+            "q", "k_cache", "v_cache", "o", "lse", "block_table", "seq_lens", "workspace")]
+        + [("workspace_bytes", ctypes.c_size_t)]
+        + [(n, ctypes.c_int64) for n in (
+            "B", "Hq", "Hkv", "D", "num_pages", "page_size", "max_pages", "block_table_stride")]
+        + [("q_strides", ctypes.c_int64 * 2), ("cache_strides", ctypes.c_int64 * 3),
+           ("scale", ctypes.c_float), ("dtype", ctypes.c_int32)])
+
+
+class FrsaPromptArgs(ctypes.Structure):
+    """Mirror of ``frsa_prompt_args`` (include/frsa.h)."""
+
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "lse", "cu_seqlens")]
+        + [(n, ctypes.c_int64) for n in ("T", "B", "Hq", "Hkv", "D")]
+        + [("q_strides", ctypes.c_int64 * 2), ("k_strides", ctypes.c_int64 * 2),
+           ("v_strides", ctypes.c_int64 * 2), ("scale", ctypes.c_float),
+           ("dtype", ctypes.c_int32)])
+
+
 class FrsaError(RuntimeError):
     """A non-zero status returned by the C ABI."""
 
@@ -175,6 +218,13 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.frsa_bwd_noalloc.restype = ctypes.c_int
     lib.frsa_bwd_noalloc_max_elements.argtypes = []
     lib.frsa_bwd_noalloc_max_elements.restype = ctypes.c_size_t
+    for name, args in (("frsa_paged_append", FrsaPagedAppendArgs),
+                       ("frsa_paged_decode", FrsaPagedDecodeArgs),
+                       ("frsa_prompt_fwd", FrsaPromptArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.frsa_paged_decode_workspace_bytes.argtypes = []
+    lib.frsa_paged_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.frsa_last_error_detail.argtypes = []
     lib.frsa_last_error_detail.restype = ctypes.c_char_p
     lib.frsa_abi_version.argtypes = []

@@ -85,6 +85,8 @@ def _ext():
         ext = build_torch_ext()
         addr = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
         ext.bind(addr(lib.frsa_fwd), addr(lib.frsa_bwd), addr(lib.frsa_bwd_workspace_bytes))
+        ext.bind_serving(addr(lib.frsa_paged_append), addr(lib.frsa_paged_decode),
+                         addr(lib.frsa_paged_decode_workspace_bytes), addr(lib.frsa_prompt_fwd))
         _EXT = ext
     return _EXT
 

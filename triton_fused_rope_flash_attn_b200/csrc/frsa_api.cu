@@ -19,6 +19,8 @@
 #include "frsa_tf32.cu"
 #include "frsa_qkv.cu"
 #include "frsa_convert.cu"
+#include "frsa_paged.cu"
+#include "frsa_prompt.cu"
 
 namespace frsa {
 
@@ -297,6 +299,9 @@ const char* frsa_strerror(int code) {
     case FRSA_ERR_SCRATCH_LIMIT:
       return "frsa: B*H*N*D exceeds the built-in scratch of frsa_bwd_noalloc "
              "(see frsa_bwd_noalloc_max_elements)";
+    case FRSA_ERR_BAD_INDEX:
+      return "frsa: a kernel met an index (page, length, position or sequence boundary) outside "
+             "its tensor";
     default: return "frsa: unknown error";
   }
 }
@@ -509,12 +514,14 @@ int frsa_query_status(void) {
   if (st != 0) {
     const int zero = 0;
     cudaMemcpyToSymbol(frsa::g_dev_status, &zero, sizeof(int));
-    return FRSA_ERR_DEVICE_TIMEOUT;
+    return st == frsa::FRSA_DEV_INDEX ? FRSA_ERR_BAD_INDEX : FRSA_ERR_DEVICE_TIMEOUT;
   }
   return FRSA_OK;
 }
 
 }  // extern "C"
 
-// The allocation-free backward entry point (uses the helpers above).
+// The serving entry points and the allocation-free backward (they use the
+// helpers above).
+#include "frsa_serve.cu"
 #include "frsa_noalloc.cu"

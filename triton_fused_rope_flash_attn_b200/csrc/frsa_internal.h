@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 
+#include "../../include/frsa.h"
+
 namespace frsa {
 
 // Tile geometry shared by every kernel: 128-row tiles, 64-column (128-byte)
@@ -115,6 +117,15 @@ cudaError_t launch_bwd_ordered(const LaunchShape& s, const CUtensorMap& tm_q,
                                const float* cosp, const float* sinp, void* dq, void* dk, void* dv,
                                float* dq_part, int nslot, int* counters, float* delta_buf,
                                const QkRotation* rot, cudaStream_t stream);
+
+// Serving (frsa_paged.cu, frsa_prompt.cu). The arguments have been checked and
+// every stride filled in. tq: 3-D map {D, Hq, T} with box {64, G, 128 / G},
+// tk, tv: {D, Hkv, T} with box {64, 1, 128}, 128-byte swizzle.
+cudaError_t launch_paged_append(const frsa_paged_append_args& a, cudaStream_t stream);
+cudaError_t launch_paged_decode(const frsa_paged_decode_args& a, cudaStream_t stream);
+size_t decode_workspace_bytes();
+cudaError_t launch_prompt(const frsa_prompt_args& a, const CUtensorMap& tq, const CUtensorMap& tk,
+                          const CUtensorMap& tv, cudaStream_t stream);
 
 // Number of SMs of the current device (queried once per device).
 int device_sm_count();

@@ -1,0 +1,624 @@
+// Causal attention over whole packed prompts with grouped heads:
+//   o[t, h] = sum_{j <= t, same sequence} softmax_j(scale q[t, h] . k[j, h']) v[j, h'],
+// h' = h / (Hq / Hkv), q [T, Hq, D], k and v [T, Hkv, D], sequence b = tokens
+// [cu_seqlens[b], cu_seqlens[b + 1]). q and k arrive rotated.
+//
+// A query tile has 128 rows: TT = 128 / G tokens (rounded down) times the G
+// query heads that share a kv head, row = token * G + head. One tile of
+// products then serves all heads of the group, short prompts fill the rows,
+// and the causal edge wastes at most TT tokens' worth of scores per row
+// block. A unit is one or two consecutive query tiles of one (sequence, kv
+// head); a persistent CTA walks its units, both tiles of a unit share each
+// K / V load.
+//
+//   warp 0       TMA producer: the unit's query tiles, then K and V tiles of
+//                128 keys into rings of KS stages
+//   warp 1       TMEM allocator + single-thread tcgen05.mma issuer
+//   warp 2       scheduler: turns unit numbers into units (two ahead)
+//   warps 4..11  two softmax warpgroups, one per query tile (thread = row =
+//                TMEM lane)
+//
+// TMEM columns: warpgroup g uses [256 g, 256 g + 128) for the scores, over
+// which it writes P as packed 16-bit pairs, and [256 g + 128, 256 g + 256)
+// for O, which accumulates there over the unit's key tiles. The softmax base
+// is raised (and O rescaled) only when a tile's maximum exceeds it by more
+// than 2^8. The products of a tile's last keys are cut to the 16-key steps
+// that some row can see.
+//
+// Masked places: keys past a row's position get P = 0, but 0 times an
+// infinity or NaN in V (a later token's, or another sequence's in the same
+// tile) would still reach O. A row whose result is not finite is therefore
+// computed again on its own, from its visible keys alone (slow_row).
+#include "frsa_internal.h"
+#include "frsa_ptx.cuh"
+
+namespace frsa {
+
+namespace {
+
+constexpr int kPrThreads = 384;
+// Registers per thread after the split (launch: 168 each; 88 + 2 x 208 = 3 x 168).
+constexpr uint32_t kPrRegsCtl = 88, kPrRegsSoftmax = 208;
+constexpr float kPrSlack = 8.f;   // log2 headroom of the softmax base
+
+struct PromptUnit {
+  int valid;       // 0: no more units
+  int start, len;  // the sequence's first token and length
+  int tok0;        // first token (in the sequence) of query tile 0; tile 1 follows at + TT
+  int kvh;
+  int n[2];        // key tiles of each query tile (0: the tile has no tokens)
+};
+
+template <int NCH>
+struct PromptSmem {
+  static constexpr int KS = NCH == 1 ? 4 : 2;
+  uint8_t q[2][NCH][kChunkBytes];
+  uint8_t k[KS][NCH][kChunkBytes];
+  uint8_t v[KS][NCH][kChunkBytes];
+  uint64_t q_full[2], q_empty[2];
+  uint64_t k_full[KS], k_empty[KS], v_full[KS], v_empty[KS];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t unit_full[2], unit_empty[2];
+  PromptUnit unit[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct PromptParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  const int* cu;
+  long long qs[2], ks[2], vs[2];   // token and head strides
+  int T, B, Hq, Hkv, D;
+  int G, TT, ntile;   // heads per kv head, tokens per query tile, query tiles per unit
+  int nids;           // unit numbers: an upper bound of the units
+  float c2;
+};
+
+// Tokens [start, end) of sequence b, held within [0, T).
+__device__ __forceinline__ void pr_sequence(const PromptParams& p, int b, int& start, int& len) {
+  const int s = __ldg(p.cu + b), e = __ldg(p.cu + b + 1);
+  start = min(max(s, 0), p.T);
+  len = max(min(e, p.T) - start, 0);
+  if (s < 0 || e < s || e > p.T) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
+}
+__device__ __forceinline__ int pr_units_of(const PromptParams& p, int b) {
+  int start, len;
+  pr_sequence(p, b, start, len);
+  const int per = p.TT * p.ntile;
+  return (len + per - 1) / per;
+}
+
+// Unit number -> unit, by a whole warp. Up to 32 sequences the longest units
+// come first over all sequences (a unit of query block t reads about t key
+// blocks, so: by descending t); beyond that, sequence after sequence, each
+// with its longest units first.
+__device__ __forceinline__ PromptUnit pr_find_unit(const PromptParams& p, int id, int lane) {
+  PromptUnit x;
+  x.valid = 0;
+  x.kvh = id % p.Hkv;
+  int rank = id / p.Hkv;
+  int b, t;
+  if (p.B <= 32) {
+    const int nb = lane < p.B ? pr_units_of(p, lane) : 0;
+    auto at_least = [&](int lvl) {   // units with query block >= lvl (each lane its own lvl)
+      int sum = 0;
+      for (int i = 0; i < p.B; ++i) sum += max(0, __shfl_sync(0xffffffffu, nb, i) - lvl);
+      return sum;
+    };
+    int n = nb;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) n = max(n, __shfl_xor_sync(0xffffffffu, n, d));
+    if (rank >= at_least(0)) return x;
+    int lo = 0;   // the largest t with at_least(t) > rank lies in [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const int c = at_least(lo + lane * step);
+      const unsigned mask = __ballot_sync(0xffffffffu, lane * step < n && c > rank);
+      const int i = 31 - __clz(mask);
+      n = min(step, n - i * step);
+      lo += i * step;
+    }
+    t = lo;
+    rank -= at_least(t + 1);
+    const unsigned mask = __ballot_sync(0xffffffffu, nb > t);
+    b = static_cast<int>(__fns(mask, 0, rank + 1));
+  } else {
+    int lo = 0, n = p.B;
+    while (n > 1) {   // the sequence that holds `rank`, 32 runs of sequences a level
+      const int step = (n + 31) / 32;
+      const int i0 = lo + min(n, lane * step), i1 = lo + min(n, (lane + 1) * step);
+      int sum = 0;
+      for (int i = i0; i < i1; ++i) sum += pr_units_of(p, i);
+      int incl = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+      }
+      const unsigned mask = __ballot_sync(0xffffffffu, incl > rank);
+      if (mask == 0) return x;
+      const int i = __ffs(mask) - 1;
+      rank -= __shfl_sync(0xffffffffu, incl - sum, i);
+      lo = __shfl_sync(0xffffffffu, i0, i);
+      n = __shfl_sync(0xffffffffu, i1 - i0, i);
+    }
+    b = lo;
+    const int nb = pr_units_of(p, b);
+    t = nb - 1 - rank;
+  }
+  pr_sequence(p, b, x.start, x.len);
+  x.tok0 = t * p.TT * p.ntile;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int t0 = x.tok0 + g * p.TT;
+    x.n[g] = g < p.ntile && t0 < x.len ? (min(x.len, t0 + p.TT) + kTile - 1) / kTile : 0;
+  }
+  x.valid = 1;
+  return x;
+}
+
+// Keys of tile j that a query tile ending at token `last` (exclusive) can
+// see, rounded up to the products' 16-key step.
+__device__ __forceinline__ int pr_keys(int last, int j) {
+  return min(kTile, (last - j * kTile + 15) & ~15);
+}
+
+// One query row from global memory, in f32, over its visible keys only.
+template <typename T>
+__device__ __noinline__ void slow_row(const PromptParams& p, long long tq, int h, int kvh,
+                                      long long key0, int nkeys, T* orow, float* lse) {
+  const T* q = static_cast<const T*>(p.q) + tq * p.qs[0] + h * p.qs[1];
+  const T* k = static_cast<const T*>(p.k) + key0 * p.ks[0] + kvh * p.ks[1];
+  const T* v = static_cast<const T*>(p.v) + key0 * p.vs[0] + kvh * p.vs[1];
+  float acc[128];
+  const int pairs = p.D / 2;
+#pragma unroll 1
+  for (int d = 0; d < p.D; ++d) acc[d] = 0.f;
+  float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < nkeys; ++j) {
+    const uint32_t* kr = reinterpret_cast<const uint32_t*>(k + j * p.ks[0]);
+    const uint32_t* vr = reinterpret_cast<const uint32_t*>(v + j * p.vs[0]);
+    const uint32_t* qr = reinterpret_cast<const uint32_t*>(q);
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < pairs; ++d) {
+      const float2 a = Elt<T>::unpack(__ldg(qr + d)), b = Elt<T>::unpack(__ldg(kr + d));
+      s = fmaf(a.x, b.x, fmaf(a.y, b.y, s));
+    }
+    s *= p.c2;
+    const float mn = fmaxf(m, s);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float alpha = ex2(m - base), w = ex2(s - base);
+    m = mn;
+    l = l * alpha + w;
+#pragma unroll 1
+    for (int d = 0; d < pairs; ++d) {
+      const float2 x = Elt<T>::unpack(__ldg(vr + d));
+      acc[2 * d] = acc[2 * d] * alpha + w * x.x;
+      acc[2 * d + 1] = acc[2 * d + 1] * alpha + w * x.y;
+    }
+  }
+  const float inv = 1.f / l;
+#pragma unroll 1
+  for (int d = 0; d < pairs; ++d)
+    reinterpret_cast<uint32_t*>(orow)[d] = Elt<T>::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+  if (lse != nullptr) *lse = (m + log2f(l)) * 0.69314718055994531f;
+}
+
+template <typename T, int NCH>
+__global__ void __launch_bounds__(kPrThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
+  using Sm = PromptSmem<NCH>;
+  constexpr int KS = Sm::KS;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Sm* smp = aligned_smem<Sm>(smem_raw);
+  if (smp == nullptr) return;
+  Sm& sm = *smp;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int DP = (p.D + 15) & ~15;
+  volatile int* abort_flag = &sm.abort_flag;
+
+  if (threadIdx.x == 0) {
+    sm.abort_flag = 0;
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sm.q_full[s], 1);
+      mbar_init(&sm.q_empty[s], 1);
+      mbar_init(&sm.s_full[s], 1);
+      mbar_init(&sm.p_full[s], 4);
+      mbar_init(&sm.o_full[s], 1);
+      mbar_init(&sm.unit_full[s], 1);
+      mbar_init(&sm.unit_empty[s], 10);   // producer, issuer, eight softmax warps
+    }
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(&sm.k_full[s], 1);
+      mbar_init(&sm.k_empty[s], 1);
+      mbar_init(&sm.v_full[s], 1);
+      mbar_init(&sm.v_empty[s], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  // Unit i of this CTA: slot i & 1 of the unit ring, parity (i >> 1) & 1.
+  // On a wait that gave up the unit counts as the end.
+  auto take_unit = [&](int i) {
+    PromptUnit x;
+    x.valid = 0;
+    if (mbar_wait(&sm.unit_full[i & 1], (i >> 1) & 1, abort_flag)) x = sm.unit[i & 1];
+    return x;
+  };
+
+  if (warp < 4) {
+    setmaxnreg_dec<kPrRegsCtl>();
+    if (warp == 2) {
+      // ---------------------------------------------------------- scheduler
+      int i = 0;
+      for (int id = blockIdx.x;; id += gridDim.x) {
+        PromptUnit x;
+        x.valid = 0;
+        if (id < p.nids) {
+          x = pr_find_unit(p, id, lane);
+          // Tokens after the last sequence belong to none: zero output.
+          const int past = min(max(__ldg(p.cu + p.B), 0), p.T);
+          for (long long t = past + id; t < p.T; t += p.nids) {
+            uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + t * p.Hq * p.D);
+            for (int e = lane; e < p.Hq * (p.D >> 3); e += 32) row[e] = make_uint4(0u, 0u, 0u, 0u);
+            if (p.lse != nullptr)
+              for (int h = lane; h < p.Hq; h += 32)
+                p.lse[static_cast<long long>(h) * p.T + t] = -INFINITY;
+          }
+          if (!x.valid) continue;
+        }
+        mbar_wait(&sm.unit_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag);
+        if (lane == 0) {
+          sm.unit[i & 1] = x;
+          mbar_arrive(&sm.unit_full[i & 1]);
+        }
+        __syncwarp();
+        ++i;
+        if (!x.valid || *abort_flag) break;
+      }
+    } else if (warp == 0) {
+      // ---------------------------------------------------------- producer
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        const uint32_t qbytes = static_cast<uint32_t>(NCH * p.G * p.TT * 128);
+        int qf[2] = {0, 0}, kf = 0, vf = 0;   // fills issued
+        bool ok = true;
+        for (int i = 0; ok; ++i) {
+          const PromptUnit x = take_unit(i);
+          if (!x.valid) break;
+          mbar_arrive(&sm.unit_empty[i & 1]);
+          for (int g = 0; g < 2 && ok; ++g) {
+            if (x.n[g] == 0) continue;
+            if (!(ok = mbar_wait(&sm.q_empty[g], (qf[g] & 1) ^ 1, abort_flag))) break;
+            mbar_arrive_expect_tx(&sm.q_full[g], qbytes);
+            for (int c = 0; c < NCH; ++c)
+              tma_load_3d(sm.q[g][c], &tm_q, &sm.q_full[g], c * kChunkCols, x.kvh * p.G,
+                          x.start + x.tok0 + g * p.TT);
+            ++qf[g];
+          }
+          const int nmax = max(x.n[0], x.n[1]);
+          for (int j = 0; j < nmax && ok; ++j) {
+            int s = kf % KS;
+            if (!(ok = mbar_wait(&sm.k_empty[s], ((kf / KS) & 1) ^ 1, abort_flag))) break;
+            mbar_arrive_expect_tx(&sm.k_full[s], NCH * kChunkBytes);
+            for (int c = 0; c < NCH; ++c)
+              tma_load_3d(sm.k[s][c], &tm_k, &sm.k_full[s], c * kChunkCols, x.kvh,
+                          x.start + j * kTile);
+            ++kf;
+            s = vf % KS;
+            if (!(ok = mbar_wait(&sm.v_empty[s], ((vf / KS) & 1) ^ 1, abort_flag))) break;
+            mbar_arrive_expect_tx(&sm.v_full[s], NCH * kChunkBytes);
+            for (int c = 0; c < NCH; ++c)
+              tma_load_3d(sm.v[s][c], &tm_v, &sm.v_full[s], c * kChunkCols, x.kvh,
+                          x.start + j * kTile);
+            ++vf;
+          }
+        }
+        // Every load that was issued lands before the CTA may end (a wait
+        // only where some other wait gave up).
+        for (int g = 0; g < 2; ++g)
+          if (qf[g] > 0) mbar_wait_limit(&sm.q_full[g], (qf[g] - 1) & 1);
+        for (int b = 1; b <= KS; ++b) {
+          if (kf >= b) mbar_wait_limit(&sm.k_full[(kf - b) % KS], ((kf - b) / KS) & 1);
+          if (vf >= b) mbar_wait_limit(&sm.v_full[(vf - b) % KS], ((vf - b) / KS) & 1);
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        constexpr bool kBf = Elt<T>::kBf16;
+        const int ksteps = DP >> 4;
+        const uint32_t idO = idesc_f16(kBf, 128, DP, false, true);
+        auto issue_s = [&](int g, int s, int keys) {
+          const uint32_t tS = tmem + 256 * g;
+          const uint32_t idS = idesc_f16(kBf, 128, keys, false, false);
+          for (int ks = 0; ks < ksteps; ++ks) {
+            const int c = ks >> 2;
+            const uint32_t koff = (ks & 3) * 32;
+            mma_ss(tS, sw128_desc(smem_u32(sm.q[g][c]) + koff, 16, 1024),
+                   sw128_desc(smem_u32(sm.k[s][c]) + koff, 16, 1024), idS, ks > 0);
+          }
+          mma_commit(&sm.s_full[g]);
+        };
+        auto issue_pv = [&](int g, int s, bool acc, int keys) {
+          const uint32_t tS = tmem + 256 * g, tO = tS + 128;
+          for (int ks = 0; ks < keys / 16; ++ks)
+            mma_ts(tO, tS + 8 * ks, sw128_desc(smem_u32(sm.v[s][0]) + ks * 2048, kChunkBytes, 1024),
+                   idO, acc || ks > 0);
+        };
+        int qf[2] = {0, 0}, tg[2] = {0, 0};
+        int t = 0, i = 0;
+        PromptUnit x = take_unit(0);
+        auto last_of = [&](const PromptUnit& y, int g) {
+          return min(y.len, y.tok0 + (g + 1) * p.TT);
+        };
+        // A unit's scores against its first key tile.
+        auto first_scores = [&](const PromptUnit& y, int tile) {
+          const int s = tile % KS;
+          mbar_wait(&sm.k_full[s], (tile / KS) & 1, abort_flag);
+          for (int g = 0; g < 2; ++g) {
+            if (y.n[g] == 0) continue;
+            mbar_wait(&sm.q_full[g], qf[g] & 1, abort_flag);
+            ++qf[g];
+            tc_fence_after();
+            issue_s(g, s, pr_keys(last_of(y, g), 0));
+            if (y.n[g] == 1) mma_commit(&sm.q_empty[g]);
+          }
+          mma_commit(&sm.k_empty[s]);
+        };
+        if (x.valid) {
+          mbar_arrive(&sm.unit_empty[0]);
+          first_scores(x, 0);
+        }
+        while (x.valid) {
+          const int nmax = max(x.n[0], x.n[1]);
+          PromptUnit y;
+          y.valid = 0;
+          for (int j = 0; j < nmax; ++j, ++t) {
+            const int s = t % KS, s1 = (t + 1) % KS;
+            const bool more = j + 1 < nmax;
+            bool k_waited = false, v_waited = false;
+            for (int g = 0; g < 2; ++g) {
+              if (j >= x.n[g]) continue;
+              mbar_wait(&sm.p_full[g], tg[g] & 1, abort_flag);
+              ++tg[g];
+              if (!v_waited) mbar_wait(&sm.v_full[s], (t / KS) & 1, abort_flag);
+              v_waited = true;
+              tc_fence_after();
+              issue_pv(g, s, j > 0, pr_keys(last_of(x, g), j));
+              if (j + 1 == x.n[g]) {
+                mma_commit(&sm.o_full[g]);
+                continue;
+              }
+              if (!k_waited) mbar_wait(&sm.k_full[s1], ((t + 1) / KS) & 1, abort_flag);
+              k_waited = true;
+              tc_fence_after();
+              issue_s(g, s1, pr_keys(last_of(x, g), j + 1));
+              if (j + 2 == x.n[g]) mma_commit(&sm.q_empty[g]);
+            }
+            if (more) {
+              mma_commit(&sm.k_empty[s1]);
+            } else {
+              y = take_unit(i + 1);
+              if (y.valid) {
+                mbar_arrive(&sm.unit_empty[(i + 1) & 1]);
+                first_scores(y, t + 1);
+              }
+            }
+            mma_commit(&sm.v_empty[s]);
+          }
+          x = y;
+          ++i;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    setmaxnreg_inc<kPrRegsSoftmax>();
+    const int g = (warp - 4) >> 2;
+    const int wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    const float c2 = p.c2;
+    const uint32_t tS = tmem + 256 * g + lane_off, tO = tS + 128;
+    const int rtok = r / p.G, head = r - rtok * p.G;
+    int tg = 0, uo = 0;
+    for (int i = 0;; ++i) {
+      const PromptUnit x = take_unit(i);
+      if (!x.valid) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.unit_empty[i & 1]);
+      if (x.n[g] == 0) continue;
+      const int t0 = x.tok0 + g * p.TT;
+      const int tok = t0 + rtok;
+      const int last = min(x.len, t0 + p.TT);
+      const int see = min(tok, last - 1);   // the last key this row sees
+      float m2 = -INFINITY, l = 0.f;
+      for (int j = 0; j < x.n[g]; ++j, ++tg) {
+        const int keys = pr_keys(last, j);
+        const bool edge = j * kTile + kTile - 1 > t0;   // some row does not see all keys
+        mbar_wait(&sm.s_full[g], tg & 1, abort_flag);
+        tc_fence_after();
+        float sv[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c * 32 < keys) tmem_ld32(tS + c * 32, sv[c]);
+        tmem_wait_ld();
+        if (edge) {
+          const int lim = see - j * kTile;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e > lim) sv[c][e] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c * 32 < keys) {
+            float a = -INFINITY, b = -INFINITY, d = -INFINITY, e4 = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              a = fmaxf(a, fmaxf(sv[c][e], sv[c][e + 1]));
+              b = fmaxf(b, fmaxf(sv[c][e + 2], sv[c][e + 3]));
+              d = fmaxf(d, fmaxf(sv[c][e + 4], sv[c][e + 5]));
+              e4 = fmaxf(e4, fmaxf(sv[c][e + 6], sv[c][e + 7]));
+            }
+            mx = fmaxf(mx, fmaxf(fmaxf(a, b), fmaxf(d, e4)));
+          }
+        const bool up = mx * c2 > m2 + kPrSlack;
+        if (__any_sync(0xffffffffu, up)) {
+          const float mn = up ? mx * c2 : m2;
+          const float alpha = ex2(m2 - mn);   // 0 while m2 is -inf
+          l *= alpha;
+          if (j > 0) {
+#pragma unroll 1
+            for (int c16 = 0; c16 * 16 < DP; ++c16) {
+              float ov[16];
+              tmem_ld16(tO + c16 * 16, ov);
+              tmem_wait_ld();
+              uint32_t w[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(ov[e] * alpha);
+              tmem_st16(tO + c16 * 16, w);
+            }
+          }
+          m2 = mn;
+        }
+        float sp[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c * 32 < keys) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              sv[c][e] = ex2(fmaf(sv[c][e], c2, -m2));
+              sp[e & 3] += sv[c][e];
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] = Elt<T>::pack(sv[c][2 * e], sv[c][2 * e + 1]);
+            tmem_st16(tS + c * 16, pk);
+          }
+        l += (sp[0] + sp[1]) + (sp[2] + sp[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[g]);
+      }
+      // O / l once the unit's last P V has completed.
+      mbar_wait(&sm.o_full[g], uo & 1, abort_flag);
+      ++uo;
+      tc_fence_after();
+      const bool stored = rtok < p.TT && tok < x.len;
+      const int h = x.kvh * p.G + head;
+      const long long tq = x.start + tok;
+      T* orow = static_cast<T*>(p.o) + (tq * p.Hq + h) * p.D;
+      const float inv = 1.f / l;
+      bool finite = true;
+#pragma unroll 1
+      for (int c16 = 0; c16 * 16 < DP; ++c16) {
+        float v[16];
+        tmem_ld16(tO + c16 * 16, v);
+        tmem_wait_ld();
+        uint4 w[2];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          v[e] *= inv;
+          finite &= fabsf(v[e]) < INFINITY;
+        }
+        w[0] = make_uint4(Elt<T>::pack(v[0], v[1]), Elt<T>::pack(v[2], v[3]),
+                          Elt<T>::pack(v[4], v[5]), Elt<T>::pack(v[6], v[7]));
+        w[1] = make_uint4(Elt<T>::pack(v[8], v[9]), Elt<T>::pack(v[10], v[11]),
+                          Elt<T>::pack(v[12], v[13]), Elt<T>::pack(v[14], v[15]));
+        if (stored) {
+          reinterpret_cast<uint4*>(orow)[2 * c16] = w[0];
+          if (c16 * 16 + 8 < p.D) reinterpret_cast<uint4*>(orow)[2 * c16 + 1] = w[1];
+        }
+      }
+      tc_fence_before();   // O is read before this group's next arrival lets a product overwrite it
+      if (stored) {
+        float* ls = p.lse == nullptr ? nullptr : p.lse + static_cast<long long>(h) * p.T + tq;
+        if (ls != nullptr) *ls = (m2 + log2f(l)) * 0.69314718055994531f;
+        if (!finite) slow_row<T>(p, tq, h, x.kvh, x.start, tok + 1, orow, ls);
+      }
+      __syncwarp();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int NCH>
+cudaError_t launch_prompt_t(const PromptParams& p, const CUtensorMap& tq, const CUtensorMap& tk,
+                            const CUtensorMap& tv, cudaStream_t stream) {
+  const size_t smem = sizeof(PromptSmem<NCH>) + 1024;
+  auto kern = prompt_kernel<T, NCH>;
+  const cudaError_t e = set_max_dynamic_smem_once(kern, smem);
+  if (e != cudaSuccess) return e;
+  const int sms = device_sm_count();
+  kern<<<p.nids < sms ? p.nids : sms, kPrThreads, smem, stream>>>(tq, tk, tv, p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_prompt(const frsa_prompt_args& a, const CUtensorMap& tq, const CUtensorMap& tk,
+                          const CUtensorMap& tv, cudaStream_t stream) {
+  PromptParams p;
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.o = a.o;
+  p.lse = a.lse;
+  p.cu = a.cu_seqlens;
+  for (int i = 0; i < 2; ++i) {
+    p.qs[i] = a.q_strides[i];
+    p.ks[i] = a.k_strides[i];
+    p.vs[i] = a.v_strides[i];
+  }
+  p.T = static_cast<int>(a.T);
+  p.B = static_cast<int>(a.B);
+  p.Hq = static_cast<int>(a.Hq);
+  p.Hkv = static_cast<int>(a.Hkv);
+  p.D = static_cast<int>(a.D);
+  p.G = p.Hq / p.Hkv;
+  p.TT = kTile / p.G;
+  p.c2 = a.scale * 1.4426950408889634f;
+  // Two query tiles per unit share its K and V loads and keep the tensor core
+  // busy during one another's softmax; one, when two would leave SMs idle.
+  auto ids = [&](int ntile) {
+    return (static_cast<long long>(p.T) / (p.TT * ntile) + p.B) * p.Hkv;
+  };
+  p.ntile = ids(2) < device_sm_count() ? 1 : 2;
+  p.nids = static_cast<int>(ids(p.ntile));
+  const bool two = p.D > 64;
+  if (a.dtype == FRSA_DTYPE_BF16)
+    return two ? launch_prompt_t<__nv_bfloat16, 2>(p, tq, tk, tv, stream)
+               : launch_prompt_t<__nv_bfloat16, 1>(p, tq, tk, tv, stream);
+  return two ? launch_prompt_t<__half, 2>(p, tq, tk, tv, stream)
+             : launch_prompt_t<__half, 1>(p, tq, tk, tv, stream);
+}
+
+}  // namespace frsa

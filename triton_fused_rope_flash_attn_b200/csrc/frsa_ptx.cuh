@@ -17,10 +17,12 @@
 
 namespace frsa {
 
-// Device status word (0 = ok). Written only on a bounded-wait timeout. The
-// library is a single translation unit, so this is its one definition.
+// Device status word (0 = ok). Written only on a bounded-wait timeout, on too
+// little shared memory, or by the serving kernels on an index (a page, a
+// length, a table row) outside its tensor. The library is a single
+// translation unit, so this is its one definition.
 __device__ int g_dev_status = 0;
-enum : int { FRSA_DEV_TIMEOUT = 1, FRSA_DEV_SMEM = 2 };
+enum : int { FRSA_DEV_TIMEOUT = 1, FRSA_DEV_SMEM = 2, FRSA_DEV_INDEX = 3 };
 
 // 1024-byte-aligned view of the dynamic shared memory, or nullptr (status
 // FRSA_DEV_SMEM recorded) when the aligned struct would not fit the launch's
@@ -174,6 +176,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     atomicExch(&g_dev_status, FRSA_DEV_TIMEOUT);
   }
   return false;
+}
+
+// Wait without regard to the abort flag (for loads still in flight when a CTA
+// gives up), with the same limit.
+__device__ __forceinline__ void mbar_wait_limit(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_test(bar, parity) && globaltimer() - t0 < FRSA_WAIT_LIMIT_NS) {
+  }
 }
 
 // ---------------------------------------------------------------- global flags

@@ -10,11 +10,15 @@
 // layer turns a non-zero code into FrsaError, as it does for direct C-ABI
 // calls.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <cmath>
 #include <cstdint>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "frsa.h"
 
@@ -174,6 +178,266 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, int64_t> bwd(
   return {dq, dk, dv, rc};
 }
 
+// ---------------------------------------------------------------- serving
+
+using AppendFn = int (*)(const frsa_paged_append_args*, void*);
+using DecodeFn = int (*)(const frsa_paged_decode_args*, void*);
+using DecodeWsFn = size_t (*)();
+using PromptFn = int (*)(const frsa_prompt_args*, void*);
+
+AppendFn g_append = nullptr;
+DecodeFn g_decode = nullptr;
+DecodeWsFn g_decode_ws = nullptr;
+PromptFn g_prompt = nullptr;
+
+void bind_serving(int64_t append, int64_t decode, int64_t decode_ws, int64_t prompt) {
+  g_append = reinterpret_cast<AppendFn>(append);
+  g_decode = reinterpret_cast<DecodeFn>(decode);
+  g_decode_ws = reinterpret_cast<DecodeWsFn>(decode_ws);
+  g_prompt = reinterpret_cast<PromptFn>(prompt);
+}
+
+int32_t serve_dtype(const at::Tensor& t) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf,
+                   "the serving operators take bfloat16 or float16, got ", t.scalar_type());
+  return t.scalar_type() == at::kBFloat16 ? FRSA_DTYPE_BF16 : FRSA_DTYPE_F16;
+}
+
+// A [tokens, heads, D] tensor: on q's device, of q's type, not asking for a gradient.
+void check_tokens(const at::Tensor& t, const at::Tensor& q, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == q.device(), name,
+              " must be a CUDA tensor on q's device (there is no CPU path)");
+  TORCH_CHECK(t.dim() == 3, name, " must be [tokens, heads, D]");
+  TORCH_CHECK_TYPE(t.scalar_type() == q.scalar_type(), name, " must have q's dtype");
+  TORCH_CHECK(t.size(2) == q.size(2), name, " must have q's head dim");
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()),
+              "the serving operators have no backward: call them under torch.no_grad()");
+}
+
+void check_cache(const at::Tensor& c, const at::Tensor& q, const at::Tensor& k_cache,
+                 const char* name) {
+  TORCH_CHECK(c.is_cuda() && c.device() == q.device(), name,
+              " must be a CUDA tensor on q's device (there is no CPU path)");
+  TORCH_CHECK(c.dim() == 4 && c.size(3) == q.size(2), name,
+              " must be [pages, kv heads, page_size, D] with q's head dim");
+  TORCH_CHECK_TYPE(c.scalar_type() == q.scalar_type(), name, " must have q's dtype");
+  TORCH_CHECK(c.sizes() == k_cache.sizes() && c.strides() == k_cache.strides(),
+              "k_cache and v_cache must have the same shape and strides");
+  TORCH_CHECK(c.stride(3) == 1 && tma_strided_ok(c), name,
+              " must have a unit d stride, other strides that are multiples of 16 bytes and "
+              "16-byte aligned data");
+  TORCH_CHECK(!(c.requires_grad() && at::GradMode::is_enabled()),
+              "the serving operators have no backward: call them under torch.no_grad()");
+}
+
+// An int32 index array on q's device, contiguous.
+at::Tensor index_array(const at::Tensor& t, const at::Tensor& q, int64_t n, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == q.device(), name, " must be on q's device");
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32");
+  TORCH_CHECK(t.dim() == 1 && (n < 0 || t.size(0) == n), name, " has the wrong shape");
+  return t.contiguous();
+}
+
+at::Tensor table_array(const at::Tensor& t, const at::Tensor& q, int64_t B) {
+  TORCH_CHECK(t.is_cuda() && t.device() == q.device(), "block_table must be on q's device");
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, "block_table must be int32");
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == B && t.size(1) >= 1,
+              "block_table must be [sequences, pages per sequence]");
+  return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous();
+}
+
+// Strided [tokens, heads, D] rows are read in place where 16-byte loads and
+// TMA can address them, otherwise copied once.
+at::Tensor readable_tokens(const at::Tensor& t) {
+  if (t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0) return t;
+  bool ok = t.stride(2) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+  for (int d = 0; d < 2; ++d) ok = ok && (t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// (first, second) strides of a tensor's leading dimensions; an extent of one
+// may carry any stride, so it gets the packed one.
+template <int N>
+void lead_strides(int64_t (&dst)[N], const at::Tensor& t) {
+  int64_t packed = t.size(N);
+  for (int d = N - 1; d >= 0; --d) {
+    dst[d] = t.size(d) > 1 ? t.stride(d) : packed;
+    packed *= t.size(d);
+  }
+}
+
+float scale_of(double scale, int64_t D) {
+  return scale > 0 ? static_cast<float>(scale) : static_cast<float>(1.0 / std::sqrt(double(D)));
+}
+
+// The split decode's scratch: one per (device, stream), made and zeroed on its
+// first use there and left ready by every call, so calls on one stream share
+// it in stream order. While a graph is captured each call gets its own (its
+// zeroing is captured with it). Kept until the process ends.
+at::Tensor decode_workspace(const at::Tensor& q, c10::cuda::CUDAStream stream) {
+  const auto opts = q.options().dtype(at::kByte);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return at::zeros({static_cast<int64_t>(g_decode_ws())}, opts);
+  static std::mutex* mu = new std::mutex;
+  static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>;
+  std::lock_guard<std::mutex> lock(*mu);
+  at::Tensor& ws = (*kept)[{static_cast<int>(q.device().index()), stream.stream()}];
+  if (!ws.defined()) ws = at::zeros({static_cast<int64_t>(g_decode_ws())}, opts);
+  return ws;
+}
+
+std::tuple<at::Tensor, at::Tensor, int64_t> paged_append(
+    const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+    const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+    const at::Tensor& start_lens, const at::Tensor& cosp, const at::Tensor& sinp,
+    const c10::optional<at::Tensor>& cu_seqlens, const c10::optional<at::Tensor>& positions) {
+  TORCH_CHECK(g_append, "frsa extension: C ABI not bound (call bind_serving first)");
+  check_tokens(q_in, q_in, "q");
+  check_tokens(k_in, q_in, "k");
+  check_tokens(v_in, q_in, "v");
+  check_cache(k_cache, q_in, k_cache, "k_cache");
+  check_cache(v_cache, q_in, k_cache, "v_cache");
+  TORCH_CHECK(k_in.sizes() == v_in.sizes() && k_in.size(0) == q_in.size(0) &&
+                  k_in.size(1) == k_cache.size(1),
+              "k and v must be [tokens, kv heads, D] with q's tokens and the cache's kv heads");
+  TORCH_CHECK_TYPE(cosp.scalar_type() == at::kFloat && sinp.scalar_type() == at::kFloat,
+                   "COSP/SINP must be float32");
+  TORCH_CHECK(cosp.dim() == 2 && cosp.sizes() == sinp.sizes() && cosp.size(1) * 2 == q_in.size(2),
+              "COSP/SINP must be [N_pos, D/2]");
+  TORCH_CHECK(cosp.device() == q_in.device() && sinp.device() == q_in.device(),
+              "RoPE tables must be on the same device as Q");
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  const int64_t T = q_in.size(0), B = start_lens.numel();
+  frsa_paged_append_args a{};
+  const at::Tensor bt = table_array(block_table, q_in, B);
+  const at::Tensor sl = index_array(start_lens, q_in, -1, "start_lens");
+  at::Tensor cu, pos;
+  if (cu_seqlens.has_value()) cu = index_array(*cu_seqlens, q_in, B + 1, "cu_seqlens");
+  else TORCH_CHECK(T == B, "without cu_seqlens there is one token per sequence");
+  if (positions.has_value()) pos = index_array(*positions, q_in, T, "positions");
+  at::Tensor q_out = at::empty(q_in.sizes(), q_in.options());
+  at::Tensor k_out = at::empty(k_in.sizes(), k_in.options());
+  a.dtype = serve_dtype(q_in);
+  if (T == 0 || q_in.size(1) == 0) return {q_out, k_out, 0};
+  const at::Tensor q = readable_tokens(q_in), k = readable_tokens(k_in), v = readable_tokens(v_in);
+  const at::Tensor c = cosp.contiguous(), s = sinp.contiguous();
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.q_out = q_out.data_ptr();
+  a.k_out = k_out.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.block_table = bt.data_ptr<int32_t>();
+  a.start_lens = sl.data_ptr<int32_t>();
+  a.cu_seqlens = cu.defined() ? cu.data_ptr<int32_t>() : nullptr;
+  a.positions = pos.defined() ? pos.data_ptr<int32_t>() : nullptr;
+  a.cosp = c.data_ptr<float>();
+  a.sinp = s.data_ptr<float>();
+  a.T = T;
+  a.B = B;
+  a.Hq = q.size(1);
+  a.Hkv = k.size(1);
+  a.D = q.size(2);
+  a.n_pos = c.size(0);
+  a.num_pages = k_cache.size(0);
+  a.page_size = k_cache.size(2);
+  a.max_pages = bt.size(1);
+  a.block_table_stride = bt.size(0) > 1 ? bt.stride(0) : bt.size(1);
+  lead_strides(a.q_strides, q);
+  lead_strides(a.k_strides, k);
+  lead_strides(a.v_strides, v);
+  lead_strides(a.cache_strides, k_cache);
+  const int rc = g_append(&a, at::cuda::getCurrentCUDAStream().stream());
+  return {q_out, k_out, rc};
+}
+
+std::tuple<at::Tensor, at::Tensor, int64_t> paged_decode(
+    const at::Tensor& q_in, const at::Tensor& k_cache, const at::Tensor& v_cache,
+    const at::Tensor& block_table, const at::Tensor& seq_lens, double scale, bool with_lse) {
+  TORCH_CHECK(g_decode && g_decode_ws, "frsa extension: C ABI not bound (call bind_serving first)");
+  check_tokens(q_in, q_in, "q");
+  check_cache(k_cache, q_in, k_cache, "k_cache");
+  check_cache(v_cache, q_in, k_cache, "v_cache");
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  const int64_t B = q_in.size(0);
+  const at::Tensor bt = table_array(block_table, q_in, B);
+  const at::Tensor sl = index_array(seq_lens, q_in, B, "seq_lens");
+  at::Tensor o = at::empty(q_in.sizes(), q_in.options()), lse;
+  if (with_lse) lse = at::empty({B, q_in.size(1)}, q_in.options().dtype(at::kFloat));
+  frsa_paged_decode_args a{};
+  a.dtype = serve_dtype(q_in);
+  if (B == 0 || q_in.size(1) == 0) return {o, lse, 0};
+  const at::Tensor q = readable_tokens(q_in);
+  const c10::cuda::CUDAStream stream = at::cuda::getCurrentCUDAStream();
+  const at::Tensor ws = decode_workspace(q, stream);
+  a.q = q.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.o = o.data_ptr();
+  a.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+  a.block_table = bt.data_ptr<int32_t>();
+  a.seq_lens = sl.data_ptr<int32_t>();
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = static_cast<size_t>(ws.numel());
+  a.B = B;
+  a.Hq = q.size(1);
+  a.Hkv = k_cache.size(1);
+  a.D = q.size(2);
+  a.num_pages = k_cache.size(0);
+  a.page_size = k_cache.size(2);
+  a.max_pages = bt.size(1);
+  a.block_table_stride = bt.size(0) > 1 ? bt.stride(0) : bt.size(1);
+  lead_strides(a.q_strides, q);
+  lead_strides(a.cache_strides, k_cache);
+  a.scale = scale_of(scale, a.D);
+  const int rc = g_decode(&a, stream.stream());
+  return {o, lse, rc};
+}
+
+std::tuple<at::Tensor, at::Tensor, int64_t> prompt(const at::Tensor& q_in, const at::Tensor& k_in,
+                                                   const at::Tensor& v_in,
+                                                   const at::Tensor& cu_seqlens, double scale,
+                                                   bool with_lse) {
+  TORCH_CHECK(g_prompt, "frsa extension: C ABI not bound (call bind_serving first)");
+  check_tokens(q_in, q_in, "q");
+  check_tokens(k_in, q_in, "k");
+  check_tokens(v_in, q_in, "v");
+  TORCH_CHECK(k_in.sizes() == v_in.sizes() && k_in.size(0) == q_in.size(0),
+              "k and v must be [tokens, kv heads, D] with q's tokens");
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  const at::Tensor cu = index_array(cu_seqlens, q_in, -1, "cu_seqlens");
+  TORCH_CHECK(cu.size(0) >= 1, "cu_seqlens must hold at least one boundary");
+  const int64_t T = q_in.size(0), Hq = q_in.size(1);
+  frsa_prompt_args a{};
+  a.dtype = serve_dtype(q_in);
+  if (T == 0 || Hq == 0 || cu.size(0) == 1) {   // no sequence: every token belongs to none
+    at::Tensor o = at::zeros(q_in.sizes(), q_in.options()), lse;
+    if (with_lse) lse = at::full({Hq, T}, -INFINITY, q_in.options().dtype(at::kFloat));
+    return {o, lse, 0};
+  }
+  at::Tensor o = at::empty(q_in.sizes(), q_in.options()), lse;
+  if (with_lse) lse = at::empty({Hq, T}, q_in.options().dtype(at::kFloat));
+  const at::Tensor q = readable_tokens(q_in), k = readable_tokens(k_in), v = readable_tokens(v_in);
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.o = o.data_ptr();
+  a.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+  a.cu_seqlens = cu.data_ptr<int32_t>();
+  a.T = T;
+  a.B = cu.size(0) - 1;
+  a.Hq = Hq;
+  a.Hkv = k.size(1);
+  a.D = q.size(2);
+  lead_strides(a.q_strides, q);
+  lead_strides(a.k_strides, k);
+  lead_strides(a.v_strides, v);
+  a.scale = scale_of(scale, a.D);
+  const int rc = g_prompt(&a, at::cuda::getCurrentCUDAStream().stream());
+  return {o, lse, rc};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -181,4 +445,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind, "bind the C-ABI entry points (frsa_fwd, frsa_bwd, frsa_bwd_workspace_bytes)");
   m.def("fwd", &fwd, "forward: (o, lse, status)");
   m.def("bwd", &bwd, "backward: (dq, dk, dv, status)");
+  m.def("bind_serving", &bind_serving,
+        "bind the serving entry points (frsa_paged_append, frsa_paged_decode, "
+        "frsa_paged_decode_workspace_bytes, frsa_prompt_fwd)");
+  m.def("paged_append", &paged_append, "append to a paged cache: (q, k, status)");
+  m.def("paged_decode", &paged_decode, "one token over a paged cache: (o, lse, status)");
+  m.def("prompt", &prompt, "causal attention over packed prompts: (o, lse, status)");
 }
