@@ -28,7 +28,7 @@ bool serve_strides(int64_t (&st)[N], const int64_t (&inner)[N]) {
 
 int serve_cache(int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t bt_stride) {
   if (num_pages < 1 || page_size < 1 || max_pages < 1 || bt_stride < 0 ||
-      num_pages > (int64_t(1) << 31) || page_size > (int64_t(1) << 30) ||
+      num_pages > 0x7FFFFFFFLL || page_size > (int64_t(1) << 30) ||
       max_pages > (int64_t(1) << 30) / page_size)
     return FRSA_ERR_BAD_SHAPE;
   return FRSA_OK;
@@ -97,6 +97,12 @@ int frsa_paged_decode(const frsa_paged_decode_args* args, void* stream) {
   int rc = serve_common(a.B, a.Hq, a.Hkv, a.D, a.dtype);
   if (rc == FRSA_OK) rc = serve_cache(a.num_pages, a.page_size, a.max_pages, a.block_table_stride);
   if (rc != FRSA_OK) return rc;
+  // The kernel numbers tiles of 64 keys over all (sequence, kv head, head
+  // block) units in 31 bits, and page and slot strides in granules in 32.
+  const int64_t tiles = (a.max_pages * a.page_size + 63) / 64;
+  if (tiles > 0x7FFFFFFFLL / (a.B * a.Hkv * ((a.Hq / a.Hkv + 7) / 8)) ||
+      a.cache_strides[0] >= (int64_t(1) << 35) || a.cache_strides[2] >= (int64_t(1) << 35))
+    return FRSA_ERR_BAD_SHAPE;
   if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.o) ||
       !aligned4(a.lse) || !aligned4(a.block_table) || !aligned4(a.seq_lens) ||
       !serve_strides(a.q_strides, {a.Hq * a.D, a.D}) ||
