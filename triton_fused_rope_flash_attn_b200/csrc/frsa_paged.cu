@@ -157,16 +157,21 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 // j < seq_lens[b] of kv head h / (Hq / Hkv).
 //
 // A unit is (sequence, kv head, block of up to 8 NT of the query heads that
-// share it); its keys go in tiles of 64. The tiles of all units form one
-// sequence that is cut evenly over the CTAs, whatever the lengths are, so a
-// CTA works on the end of one unit, some whole units and the start of another.
+// share it); its keys go in tiles of 64, and the tiles of all units, in order,
+// are the work, whatever the lengths are. It is cut into one share per CTA (the
+// same number of tiles, give or take one); a share is the end of one unit, some
+// whole units and the start of another, and its part of a unit is a segment.
 // In a tile each of the CTA's four warps takes 16 keys and runs the softmax on
 // its own (running maximum, sum and output): nothing is exchanged per tile.
 // A warp reads its K and V rows with 16-byte asynchronous copies into its own
-// ring in shared memory, several tiles ahead and across unit boundaries, so
+// ring in shared memory, several tiles ahead and across units, so
 // only the warp's own wait stands between the copies and the products. Rows
 // past the sequence's end are filled with zeros by the copy itself: what the
 // cache holds there (uninitialised memory too) never enters a product.
+//
+// Little work goes otherwise: where all units cut into pieces of up to 4 tiles
+// give no more pieces than CTAs, a CTA has one piece, so short units need no
+// joining.
 //
 // Products: mma m16n8k16 with the keys (S^T = K Q^T) and then the head dim
 // (O^T = V^T P^T) as the 16 rows and 8 query heads as columns, so groups of up
@@ -177,23 +182,29 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 // as the sum of two 16-bit values (their rounding and what that left), which
 // keeps them to 2^-16 for bf16.
 //
-// Little work (all units cut into pieces of up to 4 tiles give no more pieces
-// than CTAs) is not shared out evenly: a CTA then has one piece, so short
-// units need no joining.
-//
-// A unit within one CTA is written at once. For the others each CTA leaves
-// its (m, l, o) in the workspace; the last of a unit's CTAs to arrive (a
+// A unit within one share is written at once. For the others each share leaves
+// its (m, l, o) in the workspace, and the last of the unit's CTAs to arrive (a
 // counter that it then sets back to zero) joins them in key order: the result
 // does not depend on who comes last.
+//
+// What bounds it: memory. SMs do not read at the same speed: of 296 equal
+// shares of one 131072-token sequence (8 kv heads, 537 MB) the first is done
+// after 64 us, half after 78 and the last after 97. Tried against that and not
+// faster: further, smaller shares claimed from a ticket counter (all done
+// between 80 and 94 us, but with four times the partials, whose joining took
+// the gain back, in the kernel or in a second one); a fifth warp that copies
+// for all four (a 16-row TMA box takes about 100 cycles: 122 us in all for
+// pages of 16, though 177 against 187 for 64 sequences with pages of 64) or
+// that only schedules.
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16;                        // keys of a warp in a tile
 constexpr int kDecTile = kDecWarps * kDecKeys;      // keys of a tile
 constexpr int kDecCtasPerSm = 2;
 constexpr int kDecPiece = 4;                        // tiles of a piece at most
+constexpr int kDecBatch = 8;                        // partials whose loads are in flight in a join
 constexpr int kDecMaxHeads = 16;                    // query heads of a unit at most
 constexpr int kDecMaxD = 128;
-constexpr int kDecSlot = kDecMaxHeads * kDecMaxD;   // floats of a partial o
 
 struct DecodeParams {
   const void* q;
@@ -203,9 +214,10 @@ struct DecodeParams {
   float* lse;
   const int* block_table;
   const int* seq_lens;
-  int* counters;       // [grid]
-  float* part_o;       // [2 * grid][kDecSlot], in the layout of the warps' registers
+  int* counters;       // [grid] arrivals at a unit's shares, by its first one
+  float* part_o;       // [2 * grid][slot_floats], in the layout of the warps' registers
   float* part_ml;      // [2 * grid][16][2]
+  int slot_floats;
   long long bt_stride;
   long long qs[2];     // sequence and head strides (elements)
   long long head_g;    // cache head stride in 16-byte granules
@@ -224,8 +236,6 @@ struct DecSmem {
   static constexpr int kStages = NK > 5 ? 3 : NK > 2 ? 4 : 6;
   uint8_t ring[kDecWarps][kStages][2][kRing];
   float ml[kDecWarps][2][2 * NT][32];
-  int scan[2][kDecWarps];
-  int find[3];
   int last;
 };
 
@@ -292,24 +302,70 @@ struct DecCursor {
   int first;   // number of the unit's tile 0
 };
 
-__device__ __forceinline__ bool dec_advance(const DecodeParams& p, DecCursor& c) {
-  if (++c.tile < c.ntiles) return false;
+__device__ __forceinline__ void dec_advance(const DecodeParams& p, DecCursor& c) {
+  if (++c.tile < c.ntiles) return;
   c.tile = 0;
   c.first += c.ntiles;
-  if (++c.blk < p.blocks) return true;
+  if (++c.blk < p.blocks) return;
   c.blk = 0;
-  if (++c.h < p.Hkv) return true;
+  if (++c.h < p.Hkv) return;
   c.h = 0;
   do {
     ++c.b;
     c.len = c.b < p.B ? dec_len(p, c.b) : 1;
     c.ntiles = dec_tiles(c.len);
   } while (c.ntiles == 0);
-  return true;
+}
+
+// The sequence that holds item x, an item being a tile or (by_piece) a piece
+// of one of its U units: by a whole warp, 32 runs of sequences a level. x
+// becomes the item's number in the sequence, `first` the number of the
+// sequence's first tile.
+__device__ __forceinline__ int dec_find(const DecodeParams& p, bool by_piece, int U, int& x,
+                                        int& first, int lane) {
+  int lo = 0, n = p.B;
+  first = 0;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int i0 = lo + min(n, lane * step), i1 = lo + min(n, (lane + 1) * step);
+    int tiles = 0, items = 0;
+    for (int i = i0; i < i1; ++i) {
+      const int t = dec_tiles(dec_len(p, i));
+      tiles += t * U;
+      items += (by_piece ? dec_pieces(t) : t) * U;
+    }
+    int tiles_in = tiles, items_in = items;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, tiles_in, d);
+      const int z = __shfl_up_sync(0xffffffffu, items_in, d);
+      if (lane >= d) {
+        tiles_in += y;
+        items_in += z;
+      }
+    }
+    const int i = __ffs(__ballot_sync(0xffffffffu, x < items_in)) - 1;
+    x -= __shfl_sync(0xffffffffu, items_in - items, i);
+    first += __shfl_sync(0xffffffffu, tiles_in - tiles, i);
+    lo = __shfl_sync(0xffffffffu, i0, i);
+    n = __shfl_sync(0xffffffffu, i1, i) - lo;
+  }
+  return lo;
 }
 
 // exp2 base of a running maximum (a row whose scores are all -inf has none).
 __device__ __forceinline__ float dec_base(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Waits until at most `pending` (<= N) of the warp's copy groups are in flight.
+template <int N>
+__device__ __forceinline__ void cp_async_wait_to(int pending) {
+  if constexpr (N == 0) {
+    cp_async_wait<0>();
+  } else {
+    if (pending == N) cp_async_wait<N>();
+    else cp_async_wait_to<N - 1>(pending);
+  }
+}
 
 template <typename T, int NK, int NT>
 __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
@@ -324,28 +380,78 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
   const int U = p.Hkv * p.blocks;
   const int grid = gridDim.x, cta = blockIdx.x;
 
-  // Tiles and pieces before each thread's run of sequences, and in all.
-  const int run = (p.B + kDecThreads - 1) / kDecThreads;
-  const int b0 = min(p.B, static_cast<int>(threadIdx.x) * run), b1 = min(p.B, b0 + run);
-  int tiles = 0, pieces = 0;
-  for (int b = b0; b < b1; ++b) {
+  // Tiles and pieces in all (every warp for itself).
+  int total = 0, total_pieces = 0;
+  for (int b = lane; b < p.B; b += 32) {
     const int n = dec_tiles(dec_len(p, b));
-    tiles += n;
-    pieces += dec_pieces(n);
+    total += n;
+    total_pieces += dec_pieces(n);
   }
-  int tiles_in = tiles, pieces_in = pieces;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, tiles_in, d);
-    const int y = __shfl_up_sync(0xffffffffu, pieces_in, d);
-    if (lane >= d) {
-      tiles_in += x;
-      pieces_in += y;
-    }
+  for (int d = 16; d > 0; d >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, d);
+    total_pieces += __shfl_xor_sync(0xffffffffu, total_pieces, d);
   }
-  if (lane == 31) {
-    sm.scan[0][warp] = tiles_in;
-    sm.scan[1][warp] = pieces_in;
+  total *= U;
+  total_pieces *= U;
+
+  // Sequences with nothing cached: zero output, lse -inf.
+  auto empty_sequences = [&]() {
+    for (int b = cta; b < p.B; b += grid) {
+      const int n = __ldg(p.seq_lens + b);
+      if (n > 0 && n <= p.max_len) continue;
+      if (n != 0 && threadIdx.x == 0) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
+      if (n > 0) continue;
+      for (int i = threadIdx.x; i < p.Hq * (p.D >> 3); i += kDecThreads)
+        reinterpret_cast<uint4*>(static_cast<T*>(p.o) + static_cast<long long>(b) * p.Hq * p.D)[i] =
+            make_uint4(0u, 0u, 0u, 0u);
+      if (p.lse != nullptr)
+        for (int h = threadIdx.x; h < p.Hq; h += kDecThreads)
+          p.lse[static_cast<long long>(b) * p.Hq + h] = -INFINITY;
+    }
+  };
+
+  // This CTA's tiles [begin, end): one piece of one unit, or share number cta.
+  const bool by_piece = total_pieces <= grid;
+  const int ncta = by_piece ? total_pieces : min(grid, total);
+  if (cta >= ncta) {
+    empty_sequences();
+    return;
+  }
+  const int per_share = total / ncta, longer = total - per_share * ncta;
+  auto share_begin = [&](int c) { return c * per_share + min(c, longer); };
+  auto share_of = [&](int x) {
+    return x < longer * (per_share + 1) ? x / (per_share + 1)
+                                        : longer + (x - longer * (per_share + 1)) / per_share;
+  };
+  auto locate = [&](int x, int& rem) {   // cursor at the unit of item x, `rem` its item there
+    DecCursor c;
+    int first;
+    c.b = dec_find(p, by_piece, U, x, first, lane);
+    c.len = dec_len(p, c.b);
+    c.ntiles = dec_tiles(c.len);
+    const int per = by_piece ? dec_pieces(c.ntiles) : c.ntiles;
+    const int u = x / per;
+    rem = x - u * per;
+    c.h = u / p.blocks;
+    c.blk = u - c.h * p.blocks;
+    c.first = first + u * c.ntiles;
+    c.tile = rem;
+    return c;
+  };
+  int begin, end, piece = 0, npieces = 1;
+  DecCursor cur;
+  if (by_piece) {   // pieces of a unit differ by one tile at most
+    cur = locate(cta, piece);
+    npieces = dec_pieces(cur.ntiles);
+    const int pq = cur.ntiles / npieces, pr = cur.ntiles - pq * npieces;
+    cur.tile = piece * pq + min(piece, pr);
+    begin = cur.first + cur.tile;
+    end = begin + pq + (piece < pr);
+  } else {
+    begin = share_begin(cta);
+    end = share_begin(cta + 1);
+    cur = locate(begin, cur.tile);
   }
   // Columns past D of the ring are never copied to: zero them.
   const int pad = 2 * NK - (p.D >> 3);
@@ -355,89 +461,6 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
                                 ((p.D >> 3) + i % pad) * 16) = make_uint4(0u, 0u, 0u, 0u);
   };
   if (pad != 0) zero_pad(0, S * 2 * kDecKeys);
-  __syncthreads();
-  int tiles_before = tiles_in - tiles, pieces_before = pieces_in - pieces;
-  int total = 0, total_pieces = 0;
-#pragma unroll
-  for (int w = 0; w < kDecWarps; ++w) {
-    if (w < warp) {
-      tiles_before += sm.scan[0][w];
-      pieces_before += sm.scan[1][w];
-    }
-    total += sm.scan[0][w];
-    total_pieces += sm.scan[1][w];
-  }
-  total *= U;
-  total_pieces *= U;
-
-  // Sequences with nothing cached: zero output, lse -inf.
-  for (int b = cta; b < p.B; b += grid) {
-    const int n = __ldg(p.seq_lens + b);
-    if (n > 0 && n <= p.max_len) continue;
-    if (n != 0 && threadIdx.x == 0) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
-    if (n > 0) continue;
-    for (int i = threadIdx.x; i < p.Hq * (p.D >> 3); i += kDecThreads)
-      reinterpret_cast<uint4*>(static_cast<T*>(p.o) + static_cast<long long>(b) * p.Hq * p.D)[i] =
-          make_uint4(0u, 0u, 0u, 0u);
-    if (p.lse != nullptr)
-      for (int h = threadIdx.x; h < p.Hq; h += kDecThreads)
-        p.lse[static_cast<long long>(b) * p.Hq + h] = -INFINITY;
-  }
-
-  // This CTA's tiles [begin, end). With few pieces: one piece of one unit.
-  // Else an even share of all tiles: share c begins at c q + min(c, r).
-  const bool by_piece = total_pieces <= grid;
-  const int ncta = by_piece ? total_pieces : min(grid, total);
-  if (cta >= ncta) return;
-  const int q = total / ncta, r = total - q * ncta;
-  auto share_begin = [&](int c) { return c * q + min(c, r); };
-  auto share_of = [&](int x) {
-    return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q;
-  };
-  const int at = by_piece ? cta : share_begin(cta);
-  {   // the sequence in which they lie: one thread's run holds it
-    int lo = (by_piece ? pieces_before : tiles_before) * U;
-    if (lo <= at && at < lo + (by_piece ? pieces : tiles) * U) {
-      int t0 = tiles_before * U;
-      for (int b = b0; b < b1; ++b) {
-        const int n = dec_tiles(dec_len(p, b));
-        const int w = (by_piece ? dec_pieces(n) : n) * U;
-        if (at < lo + w) {
-          sm.find[0] = b;
-          sm.find[1] = at - lo;
-          sm.find[2] = t0;
-          break;
-        }
-        lo += w;
-        t0 += n * U;
-      }
-    }
-  }
-  __syncthreads();
-  DecCursor cur;
-  cur.b = sm.find[0];
-  cur.len = dec_len(p, cur.b);
-  cur.ntiles = dec_tiles(cur.len);
-  int begin, end, piece = 0, npieces = 1;
-  {
-    npieces = dec_pieces(cur.ntiles);
-    const int per = by_piece ? npieces : cur.ntiles;
-    const int u = sm.find[1] / per, rem = sm.find[1] - u * per;
-    cur.h = u / p.blocks;
-    cur.blk = u - cur.h * p.blocks;
-    cur.first = sm.find[2] + u * cur.ntiles;
-    if (by_piece) {   // pieces of a unit differ by one tile at most
-      const int pq = cur.ntiles / npieces, pr = cur.ntiles - pq * npieces;
-      piece = rem;
-      cur.tile = piece * pq + min(piece, pr);
-      begin = cur.first + cur.tile;
-      end = begin + pq + (piece < pr);
-    } else {
-      cur.tile = rem;
-      begin = at;
-      end = share_begin(cta + 1);
-    }
-  }
 
   // The copying side runs ahead with a cursor of its own. Pages are looked up
   // one tile before their copies: one page for the warp's 16 keys where these
@@ -447,21 +470,26 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
   const uint32_t ring0 = smem_u32(&sm.ring[warp][0][0][0]);
   const uint4* const kc = static_cast<const uint4*>(p.k_cache);
   const uint4* const vc = static_cast<const uint4*>(p.v_cache);
-  const int* table = p.block_table + ahead.b * p.bt_stride;
-  long long head_off = ahead.h * p.head_g;
-  int page = 0;              // of the lane's key row (of the warp's 16 keys)
-  int slot = -1;             // in that page; < 0: no such key
-  int held = 0;              // keys of the 16 that the sequence has
+  struct Rows {
+    int page;             // of the lane's key row (rows16: of the warp's 16 keys)
+    int slot;             // in that page; < 0: no such key
+    int held;             // keys of the 16 that the sequence has
+    long long head_off;   // of the kv head, in granules
+  };
   auto look_up = [&]() {
+    Rows w;
     const int key0 = ahead.tile * kDecTile + warp * kDecKeys;
     const int key = p.rows16 ? key0 : key0 + (lane & 15);
-    held = ahead.len - key0;
-    slot = -1;
+    w.page = 0;
+    w.slot = -1;
+    w.held = ahead.len - key0;
+    w.head_off = ahead.h * p.head_g;
     if (key < ahead.len) {
       const int pi = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-      page = __ldg(table + pi);
-      slot = key - pi * p.page_size;
+      w.page = __ldg(p.block_table + ahead.b * p.bt_stride + pi);
+      w.slot = key - pi * p.page_size;
     }
+    return w;
   };
   uint32_t goff[NK];   // granule i of the lane, from its row's (rows16: its tile's) first
 #pragma unroll
@@ -469,18 +497,18 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
     const int idx = i * 32 + lane;
     goff[i] = idx % (2 * NK) + (p.rows16 ? idx / (2 * NK) * p.slot_g : 0);
   }
-  auto copy_tile = [&](int stage) {
+  auto copy_tile = [&](int stage, const Rows& w) {
     long long off = -1;
-    if (slot >= 0) {
-      if (page >= 0 && page < p.num_pages)
-        off = static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * p.page_g +
-                                     static_cast<uint64_t>(static_cast<uint32_t>(slot)) * p.slot_g) +
-              head_off;
+    if (w.slot >= 0) {
+      if (w.page >= 0 && w.page < p.num_pages)
+        off = static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(w.page)) * p.page_g +
+                                     static_cast<uint64_t>(static_cast<uint32_t>(w.slot)) * p.slot_g) +
+              w.head_off;
       else
         atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
     }
     const uint32_t dk = ring0 + stage * 2 * Sm::kRing;
-    if (p.rows16 && off >= 0 && held >= kDecKeys) {
+    if (p.rows16 && off >= 0 && w.held >= kDecKeys) {
       const uint4* ks = kc + off;
       const uint4* vs = vc + off;
 #pragma unroll
@@ -500,7 +528,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
       const int idx = i * 32 + lane;
       const int row = idx / (2 * NK), gcol = idx % (2 * NK);
       long long e = p.rows16 ? off : __shfl_sync(0xffffffffu, off, row);
-      const bool copy = e >= 0 && row < held;
+      const bool copy = e >= 0 && row < w.held;
       if (gcol * 8 < p.D) {
         e = copy ? e + goff[i] : 0;
         const uint32_t d = dk + row * Sm::kStride + gcol * 16;
@@ -509,25 +537,44 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
       }
     }
   };
-  const int steps = end - begin;
-  int copied = 0, copy_stage = 0;
-  look_up();
-  auto copy_next = [&]() {
-    if (copied < steps) {
-      copy_tile(copy_stage);
-      copy_stage = copy_stage + 1 == S ? 0 : copy_stage + 1;
-      if (++copied < steps) {
-        if (dec_advance(p, ahead)) {
-          table = p.block_table + ahead.b * p.bt_stride;
-          head_off = ahead.h * p.head_g;
-        }
-        look_up();
-      }
-    }
-    cp_async_commit();
-  };
+  int left = end - begin;         // tiles of the share that are not computed
+  int ahead_left = left;          // ... not copied
+  int ahead_of = 0, copy_stage = 0;   // tiles copied and not computed
+  Rows rows_next;
+  {   // the first tiles: their pages are looked up together
+    Rows w[S - 1];
+    const int n = min(S - 1, left);
 #pragma unroll
-  for (int i = 0; i < S - 1; ++i) copy_next();
+    for (int i = 0; i < S - 1; ++i)
+      if (i < n) {
+        if (i > 0) dec_advance(p, ahead);
+        w[i] = look_up();
+      }
+    ahead_left -= n;
+    if (ahead_left > 0) {
+      dec_advance(p, ahead);
+      rows_next = look_up();
+    }
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+      if (i < n) {
+        copy_tile(i, w[i]);
+        cp_async_commit();
+      }
+    ahead_of = copy_stage = n;
+    if (copy_stage == S) copy_stage = 0;
+  }
+  auto copy_next = [&]() {
+    if (ahead_left == 0) return;
+    copy_tile(copy_stage, rows_next);
+    cp_async_commit();
+    copy_stage = copy_stage + 1 == S ? 0 : copy_stage + 1;
+    ++ahead_of;
+    if (--ahead_left > 0) {
+      dec_advance(p, ahead);
+      rows_next = look_up();
+    }
+  };
 
   uint32_t qb[NT][NK][2];
   float o[NT][NK][4];   // O^T: rows 16 ks + quad, + 8; columns (heads) 8 nt + 2 ql, + 1
@@ -539,7 +586,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
                       (lane >> 3 & 1) * 16;
   int stage = 0;
 
-  for (int step = 0; step < steps; ++step) {
+  for (;;) {
     if (fresh) {   // a unit begins: its query heads
       const int h0 = cur.h * p.group + cur.blk * 8 * NT;
       const int rows = min(8 * NT, p.group - cur.blk * 8 * NT);
@@ -565,7 +612,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
       fresh = false;
     }
     copy_next();   // into the stage that the previous step read
-    cp_async_wait<S - 1>();
+    cp_async_wait_to<S - 1>(ahead_of - 1);
     __syncwarp();
     const int key0 = cur.tile * kDecTile + warp * kDecKeys;
     if (key0 < cur.len) {
@@ -639,14 +686,16 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
     }
     const int used = stage;
     stage = stage + 1 == S ? 0 : stage + 1;
+    --ahead_of;
+    --left;
     __syncwarp();   // the stage's rows are read before a later copy replaces them
 
-    if (cur.tile + 1 < cur.ntiles && step + 1 < steps) {
+    if (cur.tile + 1 < cur.ntiles && left > 0) {
       ++cur.tile;
       continue;
     }
-    // The unit, or this CTA's part of it, ends: the four warps' states meet in
-    // the ring stage that each has just read (the next copy into it comes
+    // The unit, or this share's part of it, ends: the four warps' states meet
+    // in the ring stage that each has just read (the next copy into it comes
     // after this), and warp w goes on with the 16-column steps w, w + 4, ...
     float* dump = reinterpret_cast<float*>(&sm.ring[warp][used][0][0]) + lane;
 #pragma unroll
@@ -704,7 +753,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
         static_cast<long long>(cur.b) * p.Hq + cur.h * p.group + cur.blk * 8 * NT;
     const int unit_end = cur.first + cur.ntiles;
     const bool whole = cur.first >= begin && unit_end <= end;
-    int parts = 1, part0 = cta;   // the CTAs that share the unit
+    // A share leaves two partials at most: of the unit that it ends (slot 2 c)
+    // and of the unit that it begins (2 c + 1, unless that is all of it).
+    // Value i of (nt, ks) of head pair nt 4 + ql lies at ((nt 4 + ql) NK 4 + ks 4
+    // + i) 8 + quad: whole 32-byte sectors, those of heads that exist alone.
+    int parts = 1, part0 = 0;
+    bool odd0 = false;
     if (!whole) {
       if (by_piece) {
         parts = npieces;
@@ -712,36 +766,39 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
       } else {
         part0 = share_of(cur.first);
         parts = share_of(unit_end - 1) - part0 + 1;
+        odd0 = share_begin(part0) != cur.first;
       }
-      // Partial o: value i of (nt, ks) at ((nt NK + ks) 4 + i) 32 + 8 ql + quad,
-      // so a head pair's values are whole 32-byte sectors and only those of
-      // heads that exist are written and read. A CTA leaves two partials at
-      // most: of the unit that it ends and of the unit that it begins.
-      const int mine = 2 * cta + (cta == part0 && cur.first > begin);
+    }
+    auto slot_of = [&](int i) { return 2 * (part0 + i) + (i == 0 && odd0); };
+    auto part_o = [&](int slot, int nt) {
+      return p.part_o + static_cast<size_t>(slot) * p.slot_floats + (nt * 4 + ql) * (NK * 32) + quad;
+    };
+    auto part_ml = [&](int slot, int nt) {
+      return reinterpret_cast<float4*>(p.part_ml + (slot * kDecMaxHeads + nt * 8 + ql * 2) * 2);
+    };
+    if (!whole) {
+      const int mine = slot_of(cta - part0);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
         if (nt * 8 + ql * 2 < rows) {
-          float* po = p.part_o + static_cast<size_t>(mine) * kDecSlot + nt * NK * 128 + 8 * ql + quad;
+          float* po = part_o(mine, nt);
 #pragma unroll
           for (int j = 0; j < kPer; ++j) {
             const int ks = warp + j * kDecWarps;
             if (ks < NK)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) po[(ks * 4 + i) * 32] = acc[nt][j][i];
+              for (int i = 0; i < 4; ++i) __stcg(po + (ks * 4 + i) * 8, acc[nt][j][i]);
           }
-          if (warp == 0 && quad < 2)
-            *reinterpret_cast<float2*>(p.part_ml +
-                                       (mine * kDecMaxHeads + nt * 8 + ql * 2 + quad) * 2) =
-                quad == 0 ? make_float2(m[nt][0], l[nt][0]) : make_float2(m[nt][1], l[nt][1]);
+          if (warp == 0 && quad == 0)
+            __stcg(part_ml(mine, nt), make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]));
         }
-      }
-      __threadfence();
     }
-    __syncthreads();   // (also: the dumped states are read before the next copies)
+    __syncthreads();   // the dumped states are read, the partial is written
     if (pad != 0) zero_pad(used * 2 * kDecKeys, 2 * kDecKeys);
     bool write = whole;
     if (!whole) {
       if (threadIdx.x == 0) {
+        __threadfence();   // (the barrier ordered the CTA's writes before it)
         const int was = atomicAdd(p.counters + part0, 1);
         sm.last = was == parts - 1;
         if (was == parts - 1) p.counters[part0] = 0;   // as it was, for the next call
@@ -750,43 +807,55 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
       __syncthreads();
       write = sm.last != 0;
       if (write) {
-        const int s0 = 2 * part0 + (!by_piece && share_begin(part0) != cur.first);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if (nt * 8 + ql * 2 >= rows) continue;
-          auto ml_of = [&](int c) {
-            return __ldcg(reinterpret_cast<const float4*>(
-                p.part_ml +
-                ((c == 0 ? s0 : 2 * (part0 + c)) * kDecMaxHeads + nt * 8 + ql * 2) * 2));
-          };
           float mt[2] = {-INFINITY, -INFINITY}, lt[2] = {0.f, 0.f};
-#pragma unroll 8
-          for (int c = 0; c < parts; ++c) {
-            const float4 x = ml_of(c);
-            mt[0] = fmaxf(mt[0], x.x);
-            mt[1] = fmaxf(mt[1], x.z);
-          }
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[nt][j][i] = 0.f;
-#pragma unroll 4
-          for (int c = 0; c < parts; ++c) {
-            const float4 x = ml_of(c);
-            const float f[2] = {ex2(x.x - dec_base(mt[0])), ex2(x.z - dec_base(mt[1]))};
-            lt[0] += x.y * f[0];
-            lt[1] += x.w * f[1];
-            const float* po = p.part_o +
-                              static_cast<size_t>(c == 0 ? s0 : 2 * (part0 + c)) * kDecSlot +
-                              nt * NK * 128 + 8 * ql + quad;
+#pragma unroll 1
+          for (int c0 = 0; c0 < parts; c0 += kDecBatch) {
+            float4 ml[kDecBatch];   // (m, l) of two heads
+            float v[kDecBatch][kPer][4];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-              const int ks = warp + j * kDecWarps;
-              if (ks < NK)
+            for (int c = 0; c < kDecBatch; ++c) {
+              const int slot = slot_of(min(c0 + c, parts - 1));
+              const float* po = part_o(slot, nt);
+              ml[c] = __ldcg(part_ml(slot, nt));
+#pragma unroll
+              for (int j = 0; j < kPer; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                  acc[nt][j][i] += __ldcg(po + (ks * 4 + i) * 32) * f[i & 1];
+                  v[c][j][i] = __ldcg(po + (min(warp + j * kDecWarps, NK - 1) * 4 + i) * 8);
             }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float mn = mt[k];
+#pragma unroll
+              for (int c = 0; c < kDecBatch; ++c)   // (past the end: the last one again)
+                mn = fmaxf(mn, k == 0 ? ml[c].x : ml[c].z);
+              const float f = ex2(mt[k] - dec_base(mn));
+              mt[k] = mn;
+              lt[k] *= f;
+#pragma unroll
+              for (int j = 0; j < kPer; ++j) {
+                acc[nt][j][k] *= f;
+                acc[nt][j][2 + k] *= f;
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < kDecBatch; ++c)
+              if (c0 + c < parts) {
+                const float f[2] = {ex2(ml[c].x - dec_base(mt[0])), ex2(ml[c].z - dec_base(mt[1]))};
+                lt[0] += ml[c].y * f[0];
+                lt[1] += ml[c].w * f[1];
+#pragma unroll
+                for (int j = 0; j < kPer; ++j)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[nt][j][i] += v[c][j][i] * f[i & 1];
+              }
           }
           m[nt][0] = mt[0];
           m[nt][1] = mt[1];
@@ -794,6 +863,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
           l[nt][1] = lt[1];
         }
       }
+      __syncthreads();   // sm.last is read
     }
     if (write) {
 #pragma unroll
@@ -821,12 +891,18 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
       }
     }
     fresh = true;
-    if (step + 1 < steps) dec_advance(p, cur);
+    if (left > 0) {
+      dec_advance(p, cur);
+      continue;
+    }
+    break;
   }
+  empty_sequences();
 }
 
 template <typename T, int NK, int NT>
-cudaError_t launch_decode_t(const DecodeParams& p, int grid, cudaStream_t stream) {
+cudaError_t launch_decode_t(DecodeParams& p, int grid, cudaStream_t stream) {
+  p.slot_floats = ((p.group < 8 * NT ? p.group : 8 * NT) + 1) / 2 * NK * 32;
   auto kern = paged_decode_kernel<T, NK, NT>;
   const size_t smem = sizeof(DecSmem<NK, NT>);
   const cudaError_t e = set_max_dynamic_smem_once(kern, smem);
@@ -836,7 +912,7 @@ cudaError_t launch_decode_t(const DecodeParams& p, int grid, cudaStream_t stream
 }
 
 template <typename T, int NT>
-cudaError_t launch_decode_nk(const DecodeParams& p, int grid, cudaStream_t stream) {
+cudaError_t launch_decode_nk(DecodeParams& p, int grid, cudaStream_t stream) {
   if (p.D <= 32) return launch_decode_t<T, 2, NT>(p, grid, stream);
   if (p.D <= 64) return launch_decode_t<T, 4, NT>(p, grid, stream);
   if (p.D <= 80) return launch_decode_t<T, 5, NT>(p, grid, stream);
@@ -858,10 +934,9 @@ cudaError_t launch_decode_heads(DecodeParams& p, int grid, cudaStream_t stream) 
 int decode_grid() { return device_sm_count() * kDecCtasPerSm; }
 
 size_t decode_counter_bytes() { return (static_cast<size_t>(decode_grid()) * 4 + 255) & ~size_t(255); }
-
-size_t decode_workspace_bytes() {
-  return decode_counter_bytes() +
-         static_cast<size_t>(2) * decode_grid() * (kDecSlot + 2 * kDecMaxHeads) * sizeof(float);
+size_t decode_workspace_bytes() {   // two partials per share
+  return decode_counter_bytes() + static_cast<size_t>(2) * decode_grid() * kDecMaxHeads *
+                                      (kDecMaxD + 2) * sizeof(float);
 }
 
 cudaError_t launch_paged_append(const frsa_paged_append_args& a, cudaStream_t stream) {
@@ -916,7 +991,7 @@ cudaError_t launch_paged_decode(const frsa_paged_decode_args& a, cudaStream_t st
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.counters = reinterpret_cast<int*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + decode_counter_bytes());
-  p.part_ml = p.part_o + static_cast<size_t>(2) * grid * kDecSlot;
+  p.part_ml = p.part_o + static_cast<size_t>(2) * grid * kDecMaxHeads * kDecMaxD;
   p.num_pages = static_cast<int>(a.num_pages);
   p.max_len = static_cast<int>(a.max_pages * a.page_size);
   p.bt_stride = a.block_table_stride;
