@@ -233,7 +233,10 @@ template <int NK, int NT>
 struct DecSmem {
   static constexpr int kStride = (2 * NK + 1) * 16;   // bytes of a row: an odd number of granules
   static constexpr int kRing = kDecKeys * kStride;    // one K or V part of a stage
-  static constexpr int kStages = NK > 5 ? 3 : NK > 2 ? 4 : 6;
+  // About 17 KB in flight per warp. More spreads the CTAs' speeds further apart
+  // (three stages at D = 128: 131072 tokens 100 against 96 us in the kernel, 64
+  // sequences of up to 8000 tokens 182 against 177).
+  static constexpr int kStages = NK > 5 ? 2 : NK > 2 ? 3 : 5;
   uint8_t ring[kDecWarps][kStages][2][kRing];
   float ml[kDecWarps][2][2 * NT][32];
   int last;
