@@ -13,8 +13,16 @@
 //
 //   warp 0       TMA producer: the unit's query tiles, then K and V tiles of
 //                128 keys into rings of KS stages
-//   warp 1       TMEM allocator + single-thread tcgen05.mma issuer
-//   warp 2       scheduler: turns unit numbers into units (two ahead)
+//   warp 1       TMEM allocator + single-thread tcgen05.mma issuer: P V and the
+//                next scores of one query tile, then of the other, so that one
+//                is in its softmax while the other's products run (with a
+//                thread per query tile both came into step: 673 against 637 us
+//                for one prompt of 8192 tokens)
+//   warp 2       scheduler: turns unit numbers into units, two ahead. The grid
+//                has one CTA per unit number; a running CTA takes over the
+//                next one that has not started (clusterlaunchcontrol), so the
+//                longest units, which come first, are shared out as SMs get
+//                free
 //   warps 4..11  two softmax warpgroups, one per query tile (thread = row =
 //                TMEM lane)
 //
@@ -22,8 +30,13 @@
 // which it writes P as packed 16-bit pairs, and [256 g + 128, 256 g + 256)
 // for O, which accumulates there over the unit's key tiles. The softmax base
 // is raised (and O rescaled) only when a tile's maximum exceeds it by more
-// than 2^8. The products of a tile's last keys are cut to the 16-key steps
+// than 2^8. P of a tile's first 64 keys is published before the rest is
+// computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
+//
+// The exponentials bound the softmax: 16 a clock and SM, as long as the
+// products at D = 128. Some of them are computed on the FMA pipe instead
+// (exp2_poly).
 //
 // Masked places: keys past a row's position get P = 0, but 0 times an
 // infinity or NaN in V (a later token's, or another sequence's in the same
@@ -40,6 +53,7 @@ constexpr int kPrThreads = 384;
 // Registers per thread after the split (launch: 168 each; 88 + 2 x 208 = 3 x 168).
 constexpr uint32_t kPrRegsCtl = 88, kPrRegsSoftmax = 208;
 constexpr float kPrSlack = 8.f;   // log2 headroom of the softmax base
+constexpr int kPrPoly = 0, kPrPolyOf = 4;   // pairs of exponentials on the FMA pipe, of how many
 
 struct PromptUnit {
   int valid;       // 0: no more units
@@ -57,8 +71,10 @@ struct PromptSmem {
   uint8_t v[KS][NCH][kChunkBytes];
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[KS], k_empty[KS], v_full[KS], v_empty[KS];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2];   // p_full: [tile][64-key half]
   uint64_t unit_full[2], unit_empty[2];
+  uint64_t next_full;
+  alignas(16) uint32_t next[4];   // answer to the request for another unit number
   PromptUnit unit[2];
   uint32_t tmem_base;
   int abort_flag;
@@ -167,6 +183,79 @@ __device__ __forceinline__ int pr_keys(int last, int j) {
   return min(kTile, (last - j * kTile + 15) & ~15);
 }
 
+// Asks for the next CTA of the grid that has not started, to run its work in
+// its place; the 16-byte answer lands in `answer`, counted on `bar`.
+__device__ __forceinline__ void request_next(uint32_t* answer, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::
+          "r"(smem_u32(answer)), "r"(smem_u32(bar))
+      : "memory");
+}
+// The taken CTA's blockIdx.x, or -1 when none was left.
+__device__ __forceinline__ int next_id(const uint32_t* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok ? static_cast<int>(x) : -1;
+}
+
+// Pairs of f32 in one 64-bit register.
+__device__ __forceinline__ uint64_t f2_make(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_get(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of both for x <= 126 on the FMA pipe: x = n + f with n the nearest integer
+// (adding 1.5 * 2^23 leaves n in the low mantissa bits), 2^f by a polynomial
+// of degree 4 with P(0) = 1, fitted to the least largest relative error on
+// [-1/2, 1/2] (linear program over 4001 points): 2.9e-6. x is held at -126.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
+  float2 x = f2_get(x2);
+  x2 = f2_make(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const uint64_t t = f2_add(x2, f2_make(12582912.f, 12582912.f));
+  const uint64_t n = f2_add(t, f2_make(-12582912.f, -12582912.f));
+  const uint64_t f = f2_fma(n, f2_make(-1.f, -1.f), x2);
+  uint64_t y = f2_make(0x1.3a1786p-7f, 0x1.3a1786p-7f);
+  y = f2_fma(y, f, f2_make(0x1.c9fcb2p-5f, 0x1.c9fcb2p-5f));
+  y = f2_fma(y, f, f2_make(0x1.ec0328p-3f, 0x1.ec0328p-3f));
+  y = f2_fma(y, f, f2_make(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+  y = f2_fma(y, f, f2_make(1.f, 1.f));
+  const float2 e = f2_get(t), v = f2_get(y);
+  return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(e.x) << 23)),
+                     __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(e.y) << 23)));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // One query row from global memory, in f32, over its visible keys only.
 template <typename T>
 __device__ __noinline__ void slow_row(const PromptParams& p, long long tq, int h, int kvh,
@@ -230,7 +319,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(&sm.q_full[s], 1);
       mbar_init(&sm.q_empty[s], 1);
       mbar_init(&sm.s_full[s], 1);
-      mbar_init(&sm.p_full[s], 4);
+      mbar_init(&sm.p_full[s][0], 4);
+      mbar_init(&sm.p_full[s][1], 4);
       mbar_init(&sm.o_full[s], 1);
       mbar_init(&sm.unit_full[s], 1);
       mbar_init(&sm.unit_empty[s], 10);   // producer, issuer, eight softmax warps
@@ -241,6 +331,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(&sm.v_full[s], 1);
       mbar_init(&sm.v_empty[s], 1);
     }
+    mbar_init(&sm.next_full, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -265,31 +356,41 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     setmaxnreg_dec<kPrRegsCtl>();
     if (warp == 2) {
       // ---------------------------------------------------------- scheduler
-      int i = 0;
-      for (int id = blockIdx.x;; id += gridDim.x) {
-        PromptUnit x;
-        x.valid = 0;
-        if (id < p.nids) {
-          x = pr_find_unit(p, id, lane);
-          // Tokens after the last sequence belong to none: zero output.
-          const int past = min(max(__ldg(p.cu + p.B), 0), p.T);
-          for (long long t = past + id; t < p.T; t += p.nids) {
-            uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + t * p.Hq * p.D);
-            for (int e = lane; e < p.Hq * (p.D >> 3); e += 32) row[e] = make_uint4(0u, 0u, 0u, 0u);
-            if (p.lse != nullptr)
-              for (int h = lane; h < p.Hq; h += 32)
-                p.lse[static_cast<long long>(h) * p.T + t] = -INFINITY;
+      int id = blockIdx.x, i = 0;
+      for (int asked = 0;; ++asked) {
+        if (lane == 0) request_next(sm.next, &sm.next_full);   // answered while this one is found
+        const PromptUnit x = pr_find_unit(p, id, lane);
+        // Tokens after the last sequence belong to none: zero output.
+        const int past = min(max(__ldg(p.cu + p.B), 0), p.T);
+        for (long long t = past + id; t < p.T; t += p.nids) {
+          uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + t * p.Hq * p.D);
+          for (int e = lane; e < p.Hq * (p.D >> 3); e += 32) row[e] = make_uint4(0u, 0u, 0u, 0u);
+          if (p.lse != nullptr)
+            for (int h = lane; h < p.Hq; h += 32)
+              p.lse[static_cast<long long>(h) * p.T + t] = -INFINITY;
+        }
+        if (x.valid) {
+          mbar_wait(&sm.unit_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag);
+          if (lane == 0) {
+            sm.unit[i & 1] = x;
+            mbar_arrive(&sm.unit_full[i & 1]);
           }
-          if (!x.valid) continue;
+          __syncwarp();
+          ++i;
         }
-        mbar_wait(&sm.unit_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag);
-        if (lane == 0) {
-          sm.unit[i & 1] = x;
-          mbar_arrive(&sm.unit_full[i & 1]);
+        if (!mbar_wait(&sm.next_full, asked & 1, abort_flag)) {
+          mbar_wait_limit(&sm.next_full, asked & 1);   // the answer lands before the CTA ends
+          break;
         }
+        id = next_id(sm.next);
+        fence_proxy_async_smem();   // read before the next answer is written
         __syncwarp();
-        ++i;
-        if (!x.valid || *abort_flag) break;
+        if (id < 0) break;
+      }
+      mbar_wait(&sm.unit_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag);
+      if (lane == 0) {
+        sm.unit[i & 1].valid = 0;
+        mbar_arrive(&sm.unit_full[i & 1]);
       }
     } else if (warp == 0) {
       // ---------------------------------------------------------- producer
@@ -357,19 +458,18 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           }
           mma_commit(&sm.s_full[g]);
         };
-        auto issue_pv = [&](int g, int s, bool acc, int keys) {
+        auto issue_pv = [&](int g, int s, bool acc, int ks0, int ks1) {
           const uint32_t tS = tmem + 256 * g, tO = tS + 128;
-          for (int ks = 0; ks < keys / 16; ++ks)
+          for (int ks = ks0; ks < ks1; ++ks)
             mma_ts(tO, tS + 8 * ks, sw128_desc(smem_u32(sm.v[s][0]) + ks * 2048, kChunkBytes, 1024),
                    idO, acc || ks > 0);
         };
-        int qf[2] = {0, 0}, tg[2] = {0, 0};
-        int t = 0, i = 0;
-        PromptUnit x = take_unit(0);
         auto last_of = [&](const PromptUnit& y, int g) {
           return min(y.len, y.tok0 + (g + 1) * p.TT);
         };
-        // A unit's scores against its first key tile.
+        int qf[2] = {0, 0}, tg[2] = {0, 0};
+        int t = 0, i = 0;
+        // A unit's scores against its first key tile (tile number `tile`).
         auto first_scores = [&](const PromptUnit& y, int tile) {
           const int s = tile % KS;
           mbar_wait(&sm.k_full[s], (tile / KS) & 1, abort_flag);
@@ -383,6 +483,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           }
           mma_commit(&sm.k_empty[s]);
         };
+        PromptUnit x = take_unit(0);
         if (x.valid) {
           mbar_arrive(&sm.unit_empty[0]);
           first_scores(x, 0);
@@ -393,27 +494,28 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           y.valid = 0;
           for (int j = 0; j < nmax; ++j, ++t) {
             const int s = t % KS, s1 = (t + 1) % KS;
-            const bool more = j + 1 < nmax;
-            bool k_waited = false, v_waited = false;
+            mbar_wait(&sm.v_full[s], (t / KS) & 1, abort_flag);
+            if (j + 1 < nmax) mbar_wait(&sm.k_full[s1], ((t + 1) / KS) & 1, abort_flag);
             for (int g = 0; g < 2; ++g) {
               if (j >= x.n[g]) continue;
-              mbar_wait(&sm.p_full[g], tg[g] & 1, abort_flag);
-              ++tg[g];
-              if (!v_waited) mbar_wait(&sm.v_full[s], (t / KS) & 1, abort_flag);
-              v_waited = true;
+              const int steps = pr_keys(last_of(x, g), j) / 16;
+              mbar_wait(&sm.p_full[g][0], tg[g] & 1, abort_flag);
               tc_fence_after();
-              issue_pv(g, s, j > 0, pr_keys(last_of(x, g), j));
+              issue_pv(g, s, j > 0, 0, min(steps, 4));
+              mbar_wait(&sm.p_full[g][1], tg[g] & 1, abort_flag);
+              tc_fence_after();
+              issue_pv(g, s, true, 4, steps);
+              ++tg[g];
               if (j + 1 == x.n[g]) {
                 mma_commit(&sm.o_full[g]);
                 continue;
               }
-              if (!k_waited) mbar_wait(&sm.k_full[s1], ((t + 1) / KS) & 1, abort_flag);
-              k_waited = true;
-              tc_fence_after();
+              // (in order after the products that read P from the same columns)
               issue_s(g, s1, pr_keys(last_of(x, g), j + 1));
               if (j + 2 == x.n[g]) mma_commit(&sm.q_empty[g]);
             }
-            if (more) {
+            mma_commit(&sm.v_empty[s]);
+            if (j + 1 < nmax) {
               mma_commit(&sm.k_empty[s1]);
             } else {
               y = take_unit(i + 1);
@@ -422,7 +524,6 @@ __global__ void __launch_bounds__(kPrThreads, 1)
                 first_scores(y, t + 1);
               }
             }
-            mma_commit(&sm.v_empty[s]);
           }
           x = y;
           ++i;
@@ -456,33 +557,32 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         const bool edge = j * kTile + kTile - 1 > t0;   // some row does not see all keys
         mbar_wait(&sm.s_full[g], tg & 1, abort_flag);
         tc_fence_after();
+        const int lim = see - j * kTile;   // the last key of the tile that this row sees
         float sv[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           if (c * 32 < keys) tmem_ld32(tS + c * 32, sv[c]);
         tmem_wait_ld();
         if (edge) {
-          const int lim = see - j * kTile;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (c * 32 + e > lim) sv[c][e] = -INFINITY;
         }
-        float mx = -INFINITY;
+        float mx;
+        {
+          float a[4] = {sv[0][0], sv[0][1], sv[0][2], sv[0][3]};
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c * 32 < keys) {
-            float a = -INFINITY, b = -INFINITY, d = -INFINITY, e4 = -INFINITY;
+          for (int c = 0; c < 4; ++c)
+            if (c * 32 < keys)
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              a = fmaxf(a, fmaxf(sv[c][e], sv[c][e + 1]));
-              b = fmaxf(b, fmaxf(sv[c][e + 2], sv[c][e + 3]));
-              d = fmaxf(d, fmaxf(sv[c][e + 4], sv[c][e + 5]));
-              e4 = fmaxf(e4, fmaxf(sv[c][e + 6], sv[c][e + 7]));
-            }
-            mx = fmaxf(mx, fmaxf(fmaxf(a, b), fmaxf(d, e4)));
-          }
+              for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  a[k] = max3(a[k], sv[c][e + 2 * k], sv[c][e + 2 * k + 1]);
+          mx = fmaxf(max3(a[0], a[1], a[2]), a[3]);
+        }
         const bool up = mx * c2 > m2 + kPrSlack;
         if (__any_sync(0xffffffffu, up)) {
           const float mn = up ? mx * c2 : m2;
@@ -502,25 +602,40 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           }
           m2 = mn;
         }
-        float sp[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t cc = f2_make(c2, c2), mm = f2_make(-m2, -m2);
+        uint64_t sp[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
           if (c * 32 < keys) {
             uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              sv[c][e] = ex2(fmaf(sv[c][e], c2, -m2));
-              sp[e & 3] += sv[c][e];
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t x = f2_fma(f2_make(sv[c][2 * e], sv[c][2 * e + 1]), cc, mm);
+              float2 y;
+              if (e % kPrPolyOf < kPrPoly) {
+                y = exp2_poly(x);
+                if (edge) {   // exactly 0 where masked
+                  if (c * 32 + 2 * e > lim) y.x = 0.f;
+                  if (c * 32 + 2 * e + 1 > lim) y.y = 0.f;
+                }
+              } else {
+                const float2 z = f2_get(x);
+                y = make_float2(ex2(z.x), ex2(z.y));
+              }
+              sp[e & 1] = f2_add(sp[e & 1], f2_make(y.x, y.y));
+              pk[e] = Elt<T>::pack(y.x, y.y);
             }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = Elt<T>::pack(sv[c][2 * e], sv[c][2 * e + 1]);
             tmem_st16(tS + c * 16, pk);
           }
-        l += (sp[0] + sp[1]) + (sp[2] + sp[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[g]);
+          if (c & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_full[g][c >> 1]);
+          }
+        }
+        const float2 s0 = f2_get(f2_add(sp[0], sp[1]));
+        l += s0.x + s0.y;
       }
       // O / l once the unit's last P V has completed.
       mbar_wait(&sm.o_full[g], uo & 1, abort_flag);
@@ -577,8 +692,7 @@ cudaError_t launch_prompt_t(const PromptParams& p, const CUtensorMap& tq, const 
   auto kern = prompt_kernel<T, NCH>;
   const cudaError_t e = set_max_dynamic_smem_once(kern, smem);
   if (e != cudaSuccess) return e;
-  const int sms = device_sm_count();
-  kern<<<p.nids < sms ? p.nids : sms, kPrThreads, smem, stream>>>(tq, tk, tv, p);
+  kern<<<p.nids, kPrThreads, smem, stream>>>(tq, tk, tv, p);
   return cudaGetLastError();
 }
 

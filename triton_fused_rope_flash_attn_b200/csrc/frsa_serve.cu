@@ -97,6 +97,7 @@ int frsa_paged_decode(const frsa_paged_decode_args* args, void* stream) {
   int rc = serve_common(a.B, a.Hq, a.Hkv, a.D, a.dtype);
   if (rc == FRSA_OK) rc = serve_cache(a.num_pages, a.page_size, a.max_pages, a.block_table_stride);
   if (rc != FRSA_OK) return rc;
+  if (!(a.scale > 0.f)) return FRSA_ERR_BAD_SHAPE;
   // The kernel numbers tiles of 64 keys over all (sequence, kv head, head
   // block) units in 31 bits, and page and slot strides in granules in 32.
   const int64_t tiles = (a.max_pages * a.page_size + 63) / 64;
@@ -123,7 +124,7 @@ int frsa_prompt_fwd(const frsa_prompt_args* args, void* stream) {
   int rc = serve_common(a.B, a.Hq, a.Hkv, a.D, a.dtype);
   if (rc != FRSA_OK) return rc;
   const int64_t G = a.Hq / a.Hkv;
-  if (a.T < 1 || a.T > (int64_t(1) << 30) || G > 128 ||
+  if (!(a.scale > 0.f) || a.T < 1 || a.T > (int64_t(1) << 30) || G > 128 ||
       (a.T / (128 / G) + a.B) * a.Hkv > 0x7FFFFFFFLL)
     return FRSA_ERR_BAD_SHAPE;
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.o) ||

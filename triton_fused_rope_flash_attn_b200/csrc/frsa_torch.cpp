@@ -266,8 +266,9 @@ void lead_strides(int64_t (&dst)[N], const at::Tensor& t) {
   }
 }
 
-float scale_of(double scale, int64_t D) {
-  return scale > 0 ? static_cast<float>(scale) : static_cast<float>(1.0 / std::sqrt(double(D)));
+float scale_of(const c10::optional<double>& scale, int64_t D) {
+  TORCH_CHECK_VALUE(!scale.has_value() || *scale > 0, "scale must be positive");
+  return static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(double(D)));
 }
 
 // The split decode's scratch: one per (device, stream), made and zeroed on its
@@ -354,7 +355,8 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_append(
 
 std::tuple<at::Tensor, at::Tensor, int64_t> paged_decode(
     const at::Tensor& q_in, const at::Tensor& k_cache, const at::Tensor& v_cache,
-    const at::Tensor& block_table, const at::Tensor& seq_lens, double scale, bool with_lse) {
+    const at::Tensor& block_table, const at::Tensor& seq_lens, const c10::optional<double>& scale,
+    bool with_lse) {
   TORCH_CHECK(g_decode && g_decode_ws, "frsa extension: C ABI not bound (call bind_serving first)");
   check_tokens(q_in, q_in, "q");
   check_cache(k_cache, q_in, k_cache, "k_cache");
@@ -397,7 +399,8 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_decode(
 
 std::tuple<at::Tensor, at::Tensor, int64_t> prompt(const at::Tensor& q_in, const at::Tensor& k_in,
                                                    const at::Tensor& v_in,
-                                                   const at::Tensor& cu_seqlens, double scale,
+                                                   const at::Tensor& cu_seqlens,
+                                                   const c10::optional<double>& scale,
                                                    bool with_lse) {
   TORCH_CHECK(g_prompt, "frsa extension: C ABI not bound (call bind_serving first)");
   check_tokens(q_in, q_in, "q");

@@ -57,8 +57,7 @@ def paged_decode_attention(q, k_cache, v_cache, block_table, seq_lens, scale=Non
     (float32 ``[B, Hq]``). The split over the cache's length is joined in a
     fixed order: equal inputs give equal bits.
     """
-    o, lse, rc = _ext().paged_decode(q, k_cache, v_cache, block_table, seq_lens,
-                                     -1.0 if scale is None else scale, return_lse)
+    o, lse, rc = _ext().paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, return_lse)
     if rc:
         _lib.check(rc, "frsa_paged_decode")
     return (o, lse) if return_lse else o
@@ -74,7 +73,7 @@ def prompt_attention(q, k, v, cu_seqlens, scale=None, return_lse: bool = False):
     (float32 ``[Hq, T]``). Tokens from ``cu_seqlens[-1]`` on belong to no
     sequence: output 0, LSE -inf.
     """
-    o, lse, rc = _ext().prompt(q, k, v, cu_seqlens, -1.0 if scale is None else scale, return_lse)
+    o, lse, rc = _ext().prompt(q, k, v, cu_seqlens, scale, return_lse)
     if rc:
         _lib.check(rc, "frsa_prompt_fwd")
     return (o, lse) if return_lse else o
