@@ -309,7 +309,9 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   Sm* smp = aligned_smem<Sm>(smem_raw);
   if (smp == nullptr) return;
   Sm& sm = *smp;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (through a shuffle: the compiler then knows that it is the same in the warp)
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
   const int DP = (p.D + 15) & ~15;
   volatile int* abort_flag = &sm.abort_flag;
 
@@ -443,26 +445,36 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
-      if (lane == 0) {
+      // The whole warp runs this; one elected lane issues. Descriptors stay in
+      // uniform registers that way: with the loop inside `lane == 0` a product
+      // was issued every 110 clocks, where it takes 64.
+      {
         constexpr bool kBf = Elt<T>::kBf16;
         const int ksteps = DP >> 4;
         const uint32_t idO = idesc_f16(kBf, 128, DP, false, true);
+        const uint64_t q_desc = sw128_desc(smem_u32(sm.q[0][0]), 16, 1024);
+        const uint64_t k_desc = sw128_desc(smem_u32(sm.k[0][0]), 16, 1024);
+        const uint64_t v_desc = sw128_desc(smem_u32(sm.v[0][0]), kChunkBytes, 1024);
+        constexpr uint64_t kTileStep = NCH * kChunkBytes >> 4;   // of the next tile in a ring
         auto issue_s = [&](int g, int s, int keys) {
           const uint32_t tS = tmem + 256 * g;
           const uint32_t idS = idesc_f16(kBf, 128, keys, false, false);
-          for (int ks = 0; ks < ksteps; ++ks) {
-            const int c = ks >> 2;
-            const uint32_t koff = (ks & 3) * 32;
-            mma_ss(tS, sw128_desc(smem_u32(sm.q[g][c]) + koff, 16, 1024),
-                   sw128_desc(smem_u32(sm.k[s][c]) + koff, 16, 1024), idS, ks > 0);
+          const uint64_t qd = q_desc + g * kTileStep, kd = k_desc + s * kTileStep;
+#pragma unroll
+          for (int ks = 0; ks < 4 * NCH; ++ks) {
+            const uint64_t off = (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2;
+            if (ks < ksteps) mma_ss_elect(tS, qd + off, kd + off, idS, ks > 0);
           }
-          mma_commit(&sm.s_full[g]);
+          mma_commit_elect(&sm.s_full[g]);
         };
         auto issue_pv = [&](int g, int s, bool acc, int ks0, int ks1) {
           const uint32_t tS = tmem + 256 * g, tO = tS + 128;
-          for (int ks = ks0; ks < ks1; ++ks)
-            mma_ts(tO, tS + 8 * ks, sw128_desc(smem_u32(sm.v[s][0]) + ks * 2048, kChunkBytes, 1024),
-                   idO, acc || ks > 0);
+          const uint64_t vd = v_desc + s * kTileStep;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int ks = ks0 + k;
+            if (ks < ks1) mma_ts_elect(tO, tS + 8 * ks, vd + ks * 128, idO, acc || ks > 0);
+          }
         };
         auto last_of = [&](const PromptUnit& y, int g) {
           return min(y.len, y.tok0 + (g + 1) * p.TT);
@@ -479,13 +491,13 @@ __global__ void __launch_bounds__(kPrThreads, 1)
             ++qf[g];
             tc_fence_after();
             issue_s(g, s, pr_keys(last_of(y, g), 0));
-            if (y.n[g] == 1) mma_commit(&sm.q_empty[g]);
+            if (y.n[g] == 1) mma_commit_elect(&sm.q_empty[g]);
           }
-          mma_commit(&sm.k_empty[s]);
+          mma_commit_elect(&sm.k_empty[s]);
         };
         PromptUnit x = take_unit(0);
         if (x.valid) {
-          mbar_arrive(&sm.unit_empty[0]);
+          if (lane == 0) mbar_arrive(&sm.unit_empty[0]);
           first_scores(x, 0);
         }
         while (x.valid) {
@@ -507,20 +519,20 @@ __global__ void __launch_bounds__(kPrThreads, 1)
               issue_pv(g, s, true, 4, steps);
               ++tg[g];
               if (j + 1 == x.n[g]) {
-                mma_commit(&sm.o_full[g]);
+                mma_commit_elect(&sm.o_full[g]);
                 continue;
               }
               // (in order after the products that read P from the same columns)
               issue_s(g, s1, pr_keys(last_of(x, g), j + 1));
-              if (j + 2 == x.n[g]) mma_commit(&sm.q_empty[g]);
+              if (j + 2 == x.n[g]) mma_commit_elect(&sm.q_empty[g]);
             }
-            mma_commit(&sm.v_empty[s]);
+            mma_commit_elect(&sm.v_empty[s]);
             if (j + 1 < nmax) {
-              mma_commit(&sm.k_empty[s1]);
+              mma_commit_elect(&sm.k_empty[s1]);
             } else {
               y = take_unit(i + 1);
               if (y.valid) {
-                mbar_arrive(&sm.unit_empty[(i + 1) & 1]);
+                if (lane == 0) mbar_arrive(&sm.unit_empty[(i + 1) & 1]);
                 first_scores(y, t + 1);
               }
             }
