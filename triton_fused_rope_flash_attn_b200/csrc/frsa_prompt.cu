@@ -582,8 +582,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
             for (int e = 0; e < 32; ++e)
               if (c * 32 + e > lim) sv[c][e] = -INFINITY;
         }
-        float mx;
-        {
+        auto row_max = [&]() {
           float a[4] = {sv[0][0], sv[0][1], sv[0][2], sv[0][3]};
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -593,59 +592,73 @@ __global__ void __launch_bounds__(kPrThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                   a[k] = max3(a[k], sv[c][e + 2 * k], sv[c][e + 2 * k + 1]);
-          mx = fmaxf(max3(a[0], a[1], a[2]), a[3]);
-        }
-        const bool up = mx * c2 > m2 + kPrSlack;
-        if (__any_sync(0xffffffffu, up)) {
-          const float mn = up ? mx * c2 : m2;
-          const float alpha = ex2(m2 - mn);   // 0 while m2 is -inf
-          l *= alpha;
-          if (j > 0) {
-#pragma unroll 1
-            for (int c16 = 0; c16 * 16 < DP; ++c16) {
-              float ov[16];
-              tmem_ld16(tO + c16 * 16, ov);
-              tmem_wait_ld();
-              uint32_t w[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(ov[e] * alpha);
-              tmem_st16(tO + c16 * 16, w);
-            }
-          }
-          m2 = mn;
-        }
-        const uint64_t cc = f2_make(c2, c2), mm = f2_make(-m2, -m2);
+          return fmaxf(max3(a[0], a[1], a[2]), a[3]);
+        };
+        // P of 32 keys as packed pairs.
         uint64_t sp[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+        auto exps = [&](int c, uint32_t(&pk)[16]) {
+          const uint64_t cc = f2_make(c2, c2), mm = f2_make(-m2, -m2);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * 32 < keys) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint64_t x = f2_fma(f2_make(sv[c][2 * e], sv[c][2 * e + 1]), cc, mm);
-              float2 y;
-              if (e % kPrPolyOf < kPrPoly) {
-                y = exp2_poly(x);
-                if (edge) {   // exactly 0 where masked
-                  if (c * 32 + 2 * e > lim) y.x = 0.f;
-                  if (c * 32 + 2 * e + 1 > lim) y.y = 0.f;
-                }
-              } else {
-                const float2 z = f2_get(x);
-                y = make_float2(ex2(z.x), ex2(z.y));
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t x = f2_fma(f2_make(sv[c][2 * e], sv[c][2 * e + 1]), cc, mm);
+            float2 y;
+            if (e % kPrPolyOf < kPrPoly) {
+              y = exp2_poly(x);
+              if (edge) {   // exactly 0 where masked
+                if (c * 32 + 2 * e > lim) y.x = 0.f;
+                if (c * 32 + 2 * e + 1 > lim) y.y = 0.f;
               }
-              sp[e & 1] = f2_add(sp[e & 1], f2_make(y.x, y.y));
-              pk[e] = Elt<T>::pack(y.x, y.y);
+            } else {
+              const float2 z = f2_get(x);
+              y = make_float2(ex2(z.x), ex2(z.y));
             }
-            tmem_st16(tS + c * 16, pk);
+            sp[e & 1] = f2_add(sp[e & 1], f2_make(y.x, y.y));
+            pk[e] = Elt<T>::pack(y.x, y.y);
           }
-          if (c & 1) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.p_full[g][c >> 1]);
+        };
+        auto publish = [&](int h) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[g][h]);
+        };
+        // The first 64 keys' P with the base so far, while the maximum is found;
+        // then, rarely, a new base, and those keys again.
+        if (j == 0) m2 = row_max() * c2;
+        uint32_t pk0[16], pk1[16];
+        exps(0, pk0);
+        if (32 < keys) exps(1, pk1);
+        const float mx = row_max() * c2;
+        const bool up = mx > m2 + kPrSlack;
+        if (__any_sync(0xffffffffu, up)) {
+          const float mn = up ? mx : m2;
+          const float alpha = ex2(m2 - mn);
+          l *= alpha;
+          m2 = mn;
+#pragma unroll 1
+          for (int c16 = 0; c16 * 16 < DP; ++c16) {
+            float ov[16];
+            tmem_ld16(tO + c16 * 16, ov);
+            tmem_wait_ld();
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(ov[e] * alpha);
+            tmem_st16(tO + c16 * 16, w);
           }
+          sp[0] = sp[1] = f2_make(0.f, 0.f);
+          exps(0, pk0);
+          if (32 < keys) exps(1, pk1);
         }
+        tmem_st16(tS, pk0);
+        if (32 < keys) tmem_st16(tS + 16, pk1);
+        publish(0);
+#pragma unroll
+        for (int c = 2; c < 4; ++c)
+          if (c * 32 < keys) {
+            exps(c, pk0);
+            tmem_st16(tS + c * 16, pk0);
+          }
+        publish(1);
         const float2 s0 = f2_get(f2_add(sp[0], sp[1]));
         l += s0.x + s0.y;
       }
