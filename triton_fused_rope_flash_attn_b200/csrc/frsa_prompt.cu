@@ -34,9 +34,14 @@
 // computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
 //
-// The exponentials bound the softmax: 16 a clock and SM, as long as the
-// products at D = 128. Some of them are computed on the FMA pipe instead
-// (exp2_poly).
+// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 513
+// us, 1070 TFLOP/s, 64 % of the card's measured rate. Per 128 keys of a query
+// tile 1.5 us of softmax (0.3 of them waits for TMEM, the rest about 700
+// instructions on a chain per row) and 0.4 us of products before the next
+// scores; the two tiles share the SM's exponentials, of which they use half,
+// and its tensor core, of which they use half too. Tried and not faster: two
+// threads per row; a fourth or an eighth of the exponentials by a polynomial
+// on the FMA pipe; a thread of its own for each tile's products.
 //
 // Masked places: keys past a row's position get P = 0, but 0 times an
 // infinity or NaN in V (a later token's, or another sequence's in the same
@@ -53,7 +58,6 @@ constexpr int kPrThreads = 384;
 // Registers per thread after the split (launch: 168 each; 88 + 2 x 208 = 3 x 168).
 constexpr uint32_t kPrRegsCtl = 88, kPrRegsSoftmax = 208;
 constexpr float kPrSlack = 8.f;   // log2 headroom of the softmax base
-constexpr int kPrPoly = 0, kPrPolyOf = 4;   // pairs of exponentials on the FMA pipe, of how many
 
 struct PromptUnit {
   int valid;       // 0: no more units
@@ -228,26 +232,6 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-// 2^x of both for x <= 126 on the FMA pipe: x = n + f with n the nearest integer
-// (adding 1.5 * 2^23 leaves n in the low mantissa bits), 2^f by a polynomial
-// of degree 4 with P(0) = 1, fitted to the least largest relative error on
-// [-1/2, 1/2] (linear program over 4001 points): 2.9e-6. x is held at -126.
-__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
-  float2 x = f2_get(x2);
-  x2 = f2_make(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const uint64_t t = f2_add(x2, f2_make(12582912.f, 12582912.f));
-  const uint64_t n = f2_add(t, f2_make(-12582912.f, -12582912.f));
-  const uint64_t f = f2_fma(n, f2_make(-1.f, -1.f), x2);
-  uint64_t y = f2_make(0x1.3a1786p-7f, 0x1.3a1786p-7f);
-  y = f2_fma(y, f, f2_make(0x1.c9fcb2p-5f, 0x1.c9fcb2p-5f));
-  y = f2_fma(y, f, f2_make(0x1.ec0328p-3f, 0x1.ec0328p-3f));
-  y = f2_fma(y, f, f2_make(0x1.62e12cp-1f, 0x1.62e12cp-1f));
-  y = f2_fma(y, f, f2_make(1.f, 1.f));
-  const float2 e = f2_get(t), v = f2_get(y);
-  return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(e.x) << 23)),
-                     __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(e.y) << 23)));
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -570,50 +554,44 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         mbar_wait(&sm.s_full[g], tg & 1, abort_flag);
         tc_fence_after();
         const int lim = see - j * kTile;   // the last key of the tile that this row sees
-        float sv[4][32];
+        // 64 scores at a time: with 96 or 128 in registers the compiler has none
+        // left to overlap the exponentials (526 and 557 against 513 us for one
+        // prompt of 8192 tokens).
+        float sv[2][32];
+        auto load = [&](int h) {
+          if (h * 64 < keys) tmem_ld32(tS + h * 64, sv[0]);
+          if (h * 64 + 32 < keys) tmem_ld32(tS + h * 64 + 32, sv[1]);
+          tmem_wait_ld();
+          if (edge) {   // (columns that were not loaded lie past lim)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c * 32 < keys) tmem_ld32(tS + c * 32, sv[c]);
-        tmem_wait_ld();
-        if (edge) {
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e > lim) sv[c][e] = -INFINITY;
-        }
-        auto row_max = [&]() {
+              for (int e = 0; e < 32; ++e)
+                if (h * 64 + c * 32 + e > lim) sv[c][e] = -INFINITY;
+          }
+        };
+        auto half_max = [&]() {
           float a[4] = {sv[0][0], sv[0][1], sv[0][2], sv[0][3]};
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c * 32 < keys)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int e = 0; e < 32; e += 8)
+            for (int e = 0; e < 32; e += 8)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  a[k] = max3(a[k], sv[c][e + 2 * k], sv[c][e + 2 * k + 1]);
+              for (int k = 0; k < 4; ++k)
+                a[k] = max3(a[k], sv[c][e + 2 * k], sv[c][e + 2 * k + 1]);
           return fmaxf(max3(a[0], a[1], a[2]), a[3]);
         };
         // P of 32 keys as packed pairs.
-        uint64_t sp[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+        uint64_t sp[2];
         auto exps = [&](int c, uint32_t(&pk)[16]) {
           const uint64_t cc = f2_make(c2, c2), mm = f2_make(-m2, -m2);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const uint64_t x = f2_fma(f2_make(sv[c][2 * e], sv[c][2 * e + 1]), cc, mm);
-            float2 y;
-            if (e % kPrPolyOf < kPrPoly) {
-              y = exp2_poly(x);
-              if (edge) {   // exactly 0 where masked
-                if (c * 32 + 2 * e > lim) y.x = 0.f;
-                if (c * 32 + 2 * e + 1 > lim) y.y = 0.f;
-              }
-            } else {
-              const float2 z = f2_get(x);
-              y = make_float2(ex2(z.x), ex2(z.y));
-            }
-            sp[e & 1] = f2_add(sp[e & 1], f2_make(y.x, y.y));
-            pk[e] = Elt<T>::pack(y.x, y.y);
+            const float2 z = f2_get(x);
+            const float y0 = ex2(z.x), y1 = ex2(z.y);
+            sp[e & 1] = f2_add(sp[e & 1], f2_make(y0, y1));
+            pk[e] = Elt<T>::pack(y0, y1);
           }
         };
         auto publish = [&](int h) {
@@ -622,19 +600,28 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.p_full[g][h]);
         };
-        // The first 64 keys' P with the base so far, while the maximum is found;
-        // then, rarely, a new base, and those keys again.
-        if (j == 0) m2 = row_max() * c2;
+        // The first 64 keys' P with the base so far, then the maximum of the rest;
+        // rarely, a new base, and those keys again.
         uint32_t pk0[16], pk1[16];
-        exps(0, pk0);
-        if (32 < keys) exps(1, pk1);
-        const float mx = row_max() * c2;
-        const bool up = mx > m2 + kPrSlack;
-        if (__any_sync(0xffffffffu, up)) {
-          const float mn = up ? mx : m2;
+#pragma unroll 1
+        for (;;) {
+          load(0);
+          float mx = half_max();
+          if (m2 == -INFINITY) m2 = mx * c2;   // (the unit's first tile)
+          sp[0] = sp[1] = f2_make(0.f, 0.f);
+          exps(0, pk0);
+          exps(1, pk1);
+          if (64 < keys) {
+            load(1);
+            mx = fmaxf(mx, half_max());
+          }
+          const bool up = mx * c2 > m2 + kPrSlack;
+          if (!__any_sync(0xffffffffu, up)) break;
+          const float mn = up ? mx * c2 : m2;
           const float alpha = ex2(m2 - mn);
           l *= alpha;
           m2 = mn;
+          if (j == 0) continue;
 #pragma unroll 1
           for (int c16 = 0; c16 * 16 < DP; ++c16) {
             float ov[16];
@@ -645,19 +632,16 @@ __global__ void __launch_bounds__(kPrThreads, 1)
             for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(ov[e] * alpha);
             tmem_st16(tO + c16 * 16, w);
           }
-          sp[0] = sp[1] = f2_make(0.f, 0.f);
-          exps(0, pk0);
-          if (32 < keys) exps(1, pk1);
         }
         tmem_st16(tS, pk0);
         if (32 < keys) tmem_st16(tS + 16, pk1);
+        if (64 < keys) exps(0, pk0);   // while the stores complete
         publish(0);
-#pragma unroll
-        for (int c = 2; c < 4; ++c)
-          if (c * 32 < keys) {
-            exps(c, pk0);
-            tmem_st16(tS + c * 16, pk0);
-          }
+        if (64 < keys) tmem_st16(tS + 32, pk0);
+        if (96 < keys) {
+          exps(1, pk1);
+          tmem_st16(tS + 48, pk1);
+        }
         publish(1);
         const float2 s0 = f2_get(f2_add(sp[0], sp[1]));
         l += s0.x + s0.y;
