@@ -15,10 +15,14 @@ namespace {
 // Token t of sequence b has index i = start_lens[b] + t - cu_seqlens[b] and
 // rotation row p (positions[t], or i): q' = R_p q, k' = R_p k in f32, rounded
 // once; k' and v go to slot i % page_size of page block_table[b][i / page_size].
-// One CTA per token. The rows of q, k and v do not depend on where the token
-// goes, so their loads are issued before the lookups (sequence, page, table
-// row), whose dependent loads they then overlap.
+// A CTA takes one token, or four where there are many. The rows of q, k and v
+// do not depend on where a token goes, so the first two rows' loads of a
+// thread are issued before the look-ups (sequence, page, table row), a
+// warp's for a token each, whose dependent loads they then overlap. What
+// bounds it: memory for many tokens (one per CTA: 48 us for 8985 tokens of 16
+// + 32 heads of 80, 161 MB; the look-ups' latency counted), the launch for few.
 constexpr int kAppendThreads = 256;
+constexpr int kAppendMost = 4;    // tokens of a CTA at most
 
 struct AppendParams {
   const void* q;
@@ -38,6 +42,7 @@ struct AppendParams {
   long long qs[2], ks[2], vs[2];   // token and head strides
   long long cs[3];                 // cache page, head and slot strides
   int B, Hq, Hkv, D, page_size;
+  int tokens;                      // of a CTA
 };
 
 // Largest b in [0, B) with cu[b] <= t (B - 1 when t is past the end), by a
@@ -70,86 +75,124 @@ __device__ __forceinline__ uint4 rotate8(uint4 x, float4 c, float4 s) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
-  const long long t = blockIdx.x;
+__global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const AppendParams p) {
+  __shared__ long long slots[kAppendMost];   // offset of the token's slot in granules; < 0: nowhere
+  __shared__ float4 turns[kAppendMost][2][16];   // its cosines and sines
   const int G = p.D >> 3;                     // 16-byte granules per row
   const int rows = p.Hq + 2 * p.Hkv;          // q heads, k heads, v heads
   const int per = kAppendThreads / G;         // rows per pass
   const int g = threadIdx.x % G, r0 = threadIdx.x / G;
-  const int lane = threadIdx.x & 31;
-  constexpr int kAhead = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t0 = static_cast<long long>(blockIdx.x) * p.tokens;
+  const int tokens = static_cast<int>(min(static_cast<long long>(p.tokens), p.T - t0));
 
-  auto source = [&](int r) -> const uint4* {
-    const void* base;
-    long long off;
-    if (r < p.Hq) {
-      base = p.q;
-      off = t * p.qs[0] + r * p.qs[1];
-    } else if (r < p.Hq + p.Hkv) {
-      base = p.k;
-      off = t * p.ks[0] + (r - p.Hq) * p.ks[1];
-    } else {
-      base = p.v;
-      off = t * p.vs[0] + (r - p.Hq - p.Hkv) * p.vs[1];
-    }
-    return reinterpret_cast<const uint4*>(static_cast<const T*>(base) + off) + g;
+  // Granule g of one row over the CTA's tokens: where it is read and written.
+  // (Row by row with the tokens inside: all but a token's slot is found once
+  // per row, 145 -> about 70 instructions per 16 bytes.)
+  struct Row {
+    const uint4* src;
+    uint4* out;          // rotated copy (q_out, k_out), or null
+    uint4* cache;        // slot 0 of page 0, or null for q
+    long long src_step;  // granules from token to token
+    int out_step;
+    bool turn;
   };
-  uint4 x[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    const int r = r0 + i * per;
-    if (r0 < per && r < rows) x[i] = *source(r);
-  }
-
-  // Where the token goes and how it is turned.
-  int b = static_cast<int>(t);
-  long long index = 0;
-  if (p.cu_seqlens != nullptr) {
-    b = find_sequence(p.cu_seqlens, p.B, t, lane);
-    index = t - __ldg(p.cu_seqlens + b);
-  }
-  const bool held = p.cu_seqlens == nullptr || (index >= 0 && t < __ldg(p.cu_seqlens + b + 1));
-  index += __ldg(p.start_lens + b);
-  const long long pos = p.positions != nullptr ? __ldg(p.positions + t) : index;
-  const bool turn = pos >= 0 && pos < p.n_pos;
-  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (turn) {
-    c = __ldg(reinterpret_cast<const float4*>(p.cosp + pos * (p.D >> 1)) + g);
-    s = __ldg(reinterpret_cast<const float4*>(p.sinp + pos * (p.D >> 1)) + g);
-  }
-  const long long page_no = index / p.page_size;
-  bool stored = held && index >= 0 && page_no < p.max_pages;
-  long long page = 0;
-  if (stored) page = __ldg(p.block_table + b * p.bt_stride + page_no);
-  const bool bad = (held && !stored) || page < 0 || page >= p.num_pages || pos < -1 ||
-                   (held && pos >= p.n_pos);
-  stored = stored && page >= 0 && page < p.num_pages;
-  if (bad && threadIdx.x == 0) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
-  const long long slot = page * p.cs[0] + (index % p.page_size) * p.cs[2];
-
-  auto finish = [&](int r, uint4 w) {
-    if (r < p.Hq) {
-      reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + (t * p.Hq + r) * p.D)[g] =
-          rotate8<T>(w, c, s);
-    } else if (r < p.Hq + p.Hkv) {
-      const int h = r - p.Hq;
-      w = rotate8<T>(w, c, s);
-      if (p.k_out != nullptr)
-        reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + (t * p.Hkv + h) * p.D)[g] = w;
-      if (stored)
-        reinterpret_cast<uint4*>(static_cast<T*>(p.k_cache) + slot + h * p.cs[1])[g] = w;
-    } else if (stored) {
-      const int h = r - p.Hq - p.Hkv;
-      reinterpret_cast<uint4*>(static_cast<T*>(p.v_cache) + slot + h * p.cs[1])[g] = w;
-    }
+  auto row_of = [&](int r) {
+    Row w;
+    const bool q = r < p.Hq, key = !q && r < p.Hq + p.Hkv;
+    const int h = q ? r : key ? r - p.Hq : r - p.Hq - p.Hkv;
+    const T* src = static_cast<const T*>(q ? p.q : key ? p.k : p.v);
+    const long long* st = q ? p.qs : key ? p.ks : p.vs;
+    w.src = reinterpret_cast<const uint4*>(src + t0 * st[0] + h * st[1]) + g;
+    w.src_step = st[0] >> 3;
+    w.out_step = (q ? p.Hq : p.Hkv) * G;
+    T* out = static_cast<T*>(q ? p.q_out : key ? p.k_out : nullptr);
+    w.out = out == nullptr ? nullptr
+                           : reinterpret_cast<uint4*>(out) + t0 * w.out_step + h * G + g;
+    w.cache = q ? nullptr
+                : reinterpret_cast<uint4*>(static_cast<T*>(key ? p.k_cache : p.v_cache) +
+                                           h * p.cs[1]) + g;
+    w.turn = q || key;
+    return w;
   };
-  if (r0 >= per) return;
+  auto load = [&](const Row& w, uint4(&x)[kAppendMost]) {
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    const int r = r0 + i * per;
-    if (r < rows) finish(r, x[i]);
+    for (int i = 0; i < kAppendMost; ++i)
+      if (i < tokens) x[i] = __ldcs(w.src + i * w.src_step);
+  };
+  // Two rows' loads are in flight.
+  const bool works = r0 < per;
+  Row ra, rb;
+  uint4 xa[kAppendMost], xb[kAppendMost];
+  if (works && r0 < rows) {
+    ra = row_of(r0);
+    load(ra, xa);
   }
-  for (int r = r0 + kAhead * per; r < rows; r += per) finish(r, *source(r));
+  if (works && r0 + per < rows) {
+    rb = row_of(r0 + per);
+    load(rb, xb);
+  }
+
+  // Where a token goes and how it is turned.
+  if (warp < tokens) {
+    const long long t = t0 + warp;
+    int b = static_cast<int>(t);
+    long long index = 0;
+    bool held = true;
+    if (p.cu_seqlens != nullptr) {
+      b = find_sequence(p.cu_seqlens, p.B, t, lane);
+      index = t - __ldg(p.cu_seqlens + b);
+      held = index >= 0 && t < __ldg(p.cu_seqlens + b + 1);
+    }
+    index += __ldg(p.start_lens + b);
+    const long long pos = p.positions != nullptr ? __ldg(p.positions + t) : index;
+    // (in 32 bits: an index past them lies outside every block table)
+    const unsigned at = held && index >= 0 && index < (1LL << 31) ? static_cast<unsigned>(index)
+                                                                  : 0xffffffffu;
+    const unsigned page_no = at / static_cast<unsigned>(p.page_size);
+    bool stored = at != 0xffffffffu && page_no < p.max_pages;
+    long long page = 0;
+    if (stored) page = __ldg(p.block_table + b * p.bt_stride + page_no);
+    const bool bad = (held && !stored) || page < 0 || page >= p.num_pages || pos < -1 ||
+                     (held && pos >= p.n_pos);
+    stored = stored && page >= 0 && page < p.num_pages;
+    if (lane == 0) {
+      if (bad) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
+      slots[warp] = stored ? (page * p.cs[0] +
+                              static_cast<long long>(at - page_no * p.page_size) * p.cs[2]) >> 3
+                           : -1;
+    }
+    const int pairs4 = p.D >> 3;   // float4s of a table row
+    float4 f = lane < 16 ? make_float4(1.f, 1.f, 1.f, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (pos >= 0 && pos < p.n_pos && (lane & 15) < pairs4)
+      f = __ldg(reinterpret_cast<const float4*>((lane < 16 ? p.cosp : p.sinp) + pos * (p.D >> 1)) +
+                (lane & 15));
+    turns[warp][lane >> 4][lane & 15] = f;
+  }
+  __syncthreads();
+
+  if (!works) return;
+  auto finish = [&](const Row& w, const uint4(&x)[kAppendMost]) {
+#pragma unroll
+    for (int i = 0; i < kAppendMost; ++i)
+      if (i < tokens) {
+        const uint4 y = w.turn ? rotate8<T>(x[i], turns[i][0][g], turns[i][1][g]) : x[i];
+        if (w.out != nullptr) w.out[i * w.out_step] = y;
+        if (w.cache != nullptr && slots[i] >= 0) w.cache[slots[i]] = y;
+      }
+  };
+  for (int r = r0; r < rows; r += 2 * per) {
+    finish(ra, xa);
+    if (r + 2 * per < rows) {
+      ra = row_of(r + 2 * per);
+      load(ra, xa);
+    }
+    if (r + per < rows) finish(rb, xb);
+    if (r + 3 * per < rows) {
+      rb = row_of(r + 3 * per);
+      load(rb, xb);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- decode
@@ -973,7 +1016,9 @@ cudaError_t launch_paged_append(const frsa_paged_append_args& a, cudaStream_t st
   p.Hkv = static_cast<int>(a.Hkv);
   p.D = static_cast<int>(a.D);
   p.page_size = static_cast<int>(a.page_size);
-  const unsigned grid = static_cast<unsigned>(a.T);
+  // Few tokens: a CTA each, for the shortest chain.
+  p.tokens = a.T > 4 * device_sm_count() ? kAppendMost : 1;
+  const unsigned grid = static_cast<unsigned>((a.T + p.tokens - 1) / p.tokens);
   if (a.dtype == FRSA_DTYPE_BF16)
     paged_append_kernel<__nv_bfloat16><<<grid, kAppendThreads, 0, stream>>>(p);
   else

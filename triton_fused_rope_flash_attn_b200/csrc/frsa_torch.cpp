@@ -10,6 +10,7 @@
 // layer turns a non-zero code into FrsaError, as it does for direct C-ABI
 // calls.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -266,6 +267,11 @@ void lead_strides(int64_t (&dst)[N], const at::Tensor& t) {
   }
 }
 
+// An output of q's type (or `type`) on q's device, without the dispatcher.
+at::Tensor output(at::IntArrayRef sizes, const at::Tensor& q, c10::optional<at::ScalarType> type = {}) {
+  return at::detail::empty_cuda(sizes, type.value_or(q.scalar_type()), q.device(), c10::nullopt);
+}
+
 float scale_of(const c10::optional<double>& scale, int64_t D) {
   TORCH_CHECK_VALUE(!scale.has_value() || *scale > 0, "scale must be positive");
   return static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(double(D)));
@@ -316,8 +322,8 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_append(
   if (cu_seqlens.has_value()) cu = index_array(*cu_seqlens, q_in, B + 1, "cu_seqlens");
   else TORCH_CHECK(T == B, "without cu_seqlens there is one token per sequence");
   if (positions.has_value()) pos = index_array(*positions, q_in, T, "positions");
-  at::Tensor q_out = at::empty(q_in.sizes(), q_in.options());
-  at::Tensor k_out = at::empty(k_in.sizes(), k_in.options());
+  at::Tensor q_out = output(q_in.sizes(), q_in);
+  at::Tensor k_out = output(k_in.sizes(), q_in);
   a.dtype = serve_dtype(q_in);
   if (T == 0 || q_in.size(1) == 0) return {q_out, k_out, 0};
   const at::Tensor q = readable_tokens(q_in), k = readable_tokens(k_in), v = readable_tokens(v_in);
@@ -365,8 +371,8 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_decode(
   const int64_t B = q_in.size(0);
   const at::Tensor bt = table_array(block_table, q_in, B);
   const at::Tensor sl = index_array(seq_lens, q_in, B, "seq_lens");
-  at::Tensor o = at::empty(q_in.sizes(), q_in.options()), lse;
-  if (with_lse) lse = at::empty({B, q_in.size(1)}, q_in.options().dtype(at::kFloat));
+  at::Tensor o = output(q_in.sizes(), q_in), lse;
+  if (with_lse) lse = output({B, q_in.size(1)}, q_in, at::kFloat);
   frsa_paged_decode_args a{};
   a.dtype = serve_dtype(q_in);
   if (B == 0 || q_in.size(1) == 0) return {o, lse, 0};
@@ -419,8 +425,8 @@ std::tuple<at::Tensor, at::Tensor, int64_t> prompt(const at::Tensor& q_in, const
     if (with_lse) lse = at::full({Hq, T}, -INFINITY, q_in.options().dtype(at::kFloat));
     return {o, lse, 0};
   }
-  at::Tensor o = at::empty(q_in.sizes(), q_in.options()), lse;
-  if (with_lse) lse = at::empty({Hq, T}, q_in.options().dtype(at::kFloat));
+  at::Tensor o = output(q_in.sizes(), q_in), lse;
+  if (with_lse) lse = output({Hq, T}, q_in, at::kFloat);
   const at::Tensor q = readable_tokens(q_in), k = readable_tokens(k_in), v = readable_tokens(v_in);
   a.q = q.data_ptr();
   a.k = k.data_ptr();
