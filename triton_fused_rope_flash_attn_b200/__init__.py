@@ -20,6 +20,7 @@ from .serving import (  # noqa: F401
     paged_rope_append,
     prompt_attention,
 )
+from .decoder import CausalRopeAttention, PagedKVCache  # noqa: F401
 
 __all__ = [
     "build_axial_rope_pairs",
@@ -33,4 +34,6 @@ __all__ = [
     "paged_rope_append",
     "paged_decode_attention",
     "prompt_attention",
+    "PagedKVCache",
+    "CausalRopeAttention",
 ]
