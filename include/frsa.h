@@ -264,7 +264,9 @@ int frsa_convert_out(const frsa_convert_args* args, void* stream);
  * rotation row p = positions[t] (positions NULL: p = i; p = -1: not rotated):
  * q_out[t] = R_p q[t], k_out[t] = R_p k[t] (rotated in f32, rounded once),
  * and R_p k[t], v[t] are written to the caches. q_out and k_out are
- * contiguous; k_out may be NULL. Two tokens must not share a slot. */
+ * contiguous; k_out may be NULL. Two tokens must not share a slot. Tokens
+ * outside [cu_seqlens[0], cu_seqlens[B]) belong to no sequence: they are not
+ * rotated and not stored. */
 typedef struct frsa_paged_append_args {
   const void* q;
   const void* k;
@@ -327,8 +329,9 @@ size_t frsa_paged_decode_workspace_bytes(void);
 /* Causal attention over whole packed prompts:
  * o[t, h] = sum_j softmax_j(scale q[t, h] . k[j, h']) v[j, h'] over the
  * tokens j <= t of t's sequence; q and k arrive rotated. o contiguous
- * [T, Hq, D], lse [Hq, T] (natural log) or NULL. Tokens from cu_seqlens[B] on
- * belong to no sequence: o = 0, lse = -inf. Hq / Hkv <= 128. */
+ * [T, Hq, D], lse [Hq, T] (natural log) or NULL. Tokens outside
+ * [cu_seqlens[0], cu_seqlens[B]) belong to no sequence: o = 0, lse = -inf.
+ * Hq / Hkv <= 128. */
 typedef struct frsa_prompt_args {
   const void* q;
   const void* k;

@@ -138,6 +138,11 @@ def test_prompt_tokens_of_no_sequence():
     want = prompt64(q[:41], k[:41], v[:41], [30, 11], 0.125, BF)
     check(o[:41], want[0], want[1])
     assert (o[41:] == 0).all() and (lse[:, 41:] == -math.inf).all()
+    cu = ints([9, 30, 41])
+    o, lse = frsa().prompt_attention(q, k, v, cu, return_lse=True)
+    want = prompt64(q[9:41], k[9:41], v[9:41], [21, 11], 0.125, BF)
+    check(o[9:41], want[0], want[1])
+    assert (o[:9] == 0).all() and (lse[:, :9] == -math.inf).all() and (o[41:] == 0).all()
     o, lse = frsa().prompt_attention(q, k, v, ints([0, 0, 0]), return_lse=True)
     assert (o == 0).all() and (lse == -math.inf).all()
     o, lse = frsa().prompt_attention(q, k, v, ints([0]), return_lse=True)
@@ -332,6 +337,10 @@ def test_append_index_values_outside():
     bad[:] = -1
     assert call([0, 0], bad) == 11
     assert call([0, 0], cu=ints([0, 0, 0])) == 0   # tokens of no sequence go nowhere
+    assert call([0, 0], cu=ints([2, 2, 2])) == 0
+    qr, kr = frsa().paged_rope_append(q, k, v, kc, vc, table, ints([7, 7]), cosp, sinp,
+                                      cu_seqlens=ints([2, 2, 2]))
+    assert torch.equal(qr, q) and torch.equal(kr, k) and status() == 0
     assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
     assert call([0, 0], positions=ints([40, 0])) == 11
     assert call([0, 0], positions=ints([-2, 0])) == 11

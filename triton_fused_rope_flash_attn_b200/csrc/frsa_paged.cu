@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
       held = index >= 0 && t < __ldg(p.cu_seqlens + b + 1);
     }
     index += __ldg(p.start_lens + b);
-    const long long pos = p.positions != nullptr ? __ldg(p.positions + t) : index;
+    const long long pos = !held ? -1 : p.positions != nullptr ? __ldg(p.positions + t) : index;
     // (in 32 bits: an index past them lies outside every block table)
     const unsigned at = held && index >= 0 && index < (1LL << 31) ? static_cast<unsigned>(index)
                                                                   : 0xffffffffu;
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
     long long page = 0;
     if (stored) page = __ldg(p.block_table + b * p.bt_stride + page_no);
     const bool bad = (held && !stored) || page < 0 || page >= p.num_pages || pos < -1 ||
-                     (held && pos >= p.n_pos);
+                     pos >= p.n_pos;
     stored = stored && page >= 0 && page < p.num_pages;
     if (lane == 0) {
       if (bad) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
@@ -801,8 +801,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
     const bool whole = cur.first >= begin && unit_end <= end;
     // A share leaves two partials at most: of the unit that it ends (slot 2 c)
     // and of the unit that it begins (2 c + 1, unless that is all of it).
-    // Value i of (nt, ks) of head pair nt 4 + ql lies at ((nt 4 + ql) NK 4 + ks 4
-    // + i) 8 + quad: whole 32-byte sectors, those of heads that exist alone.
+    // The four values of (nt, ks) of head pair nt 4 + ql lie at (((nt 4 + ql) NK
+    // + ks) 8 + quad) 4: 16 bytes a lane, those of heads that exist alone.
     int parts = 1, part0 = 0;
     bool odd0 = false;
     if (!whole) {
@@ -817,7 +817,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
     }
     auto slot_of = [&](int i) { return 2 * (part0 + i) + (i == 0 && odd0); };
     auto part_o = [&](int slot, int nt) {
-      return p.part_o + static_cast<size_t>(slot) * p.slot_floats + (nt * 4 + ql) * (NK * 32) + quad;
+      return reinterpret_cast<float4*>(p.part_o + static_cast<size_t>(slot) * p.slot_floats) +
+             (nt * 4 + ql) * (NK * 8) + quad;
     };
     auto part_ml = [&](int slot, int nt) {
       return reinterpret_cast<float4*>(p.part_ml + (slot * kDecMaxHeads + nt * 8 + ql * 2) * 2);
@@ -827,13 +828,13 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
         if (nt * 8 + ql * 2 < rows) {
-          float* po = part_o(mine, nt);
+          float4* po = part_o(mine, nt);
 #pragma unroll
           for (int j = 0; j < kPer; ++j) {
             const int ks = warp + j * kDecWarps;
             if (ks < NK)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) __stcg(po + (ks * 4 + i) * 8, acc[nt][j][i]);
+              __stcg(po + ks * 8, make_float4(acc[nt][j][0], acc[nt][j][1], acc[nt][j][2],
+                                              acc[nt][j][3]));
           }
           if (warp == 0 && quad == 0)
             __stcg(part_ml(mine, nt), make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]));
@@ -864,17 +865,15 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
 #pragma unroll 1
           for (int c0 = 0; c0 < parts; c0 += kDecBatch) {
             float4 ml[kDecBatch];   // (m, l) of two heads
-            float v[kDecBatch][kPer][4];
+            float4 v[kDecBatch][kPer];
 #pragma unroll
             for (int c = 0; c < kDecBatch; ++c) {
               const int slot = slot_of(min(c0 + c, parts - 1));
-              const float* po = part_o(slot, nt);
+              const float4* po = part_o(slot, nt);
               ml[c] = __ldcg(part_ml(slot, nt));
 #pragma unroll
               for (int j = 0; j < kPer; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  v[c][j][i] = __ldcg(po + (min(warp + j * kDecWarps, NK - 1) * 4 + i) * 8);
+                v[c][j] = __ldcg(po + min(warp + j * kDecWarps, NK - 1) * 8);
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -898,9 +897,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
                 lt[0] += ml[c].y * f[0];
                 lt[1] += ml[c].w * f[1];
 #pragma unroll
-                for (int j = 0; j < kPer; ++j)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) acc[nt][j][i] += v[c][j][i] * f[i & 1];
+                for (int j = 0; j < kPer; ++j) {
+                  acc[nt][j][0] += v[c][j].x * f[0];
+                  acc[nt][j][1] += v[c][j].y * f[1];
+                  acc[nt][j][2] += v[c][j].z * f[0];
+                  acc[nt][j][3] += v[c][j].w * f[1];
+                }
               }
           }
           m[nt][0] = mt[0];

@@ -346,9 +346,12 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       for (int asked = 0;; ++asked) {
         if (lane == 0) request_next(sm.next, &sm.next_full);   // answered while this one is found
         const PromptUnit x = pr_find_unit(p, id, lane);
-        // Tokens after the last sequence belong to none: zero output.
+        // Tokens before the first sequence and after the last belong to none:
+        // zero output.
         const int past = min(max(__ldg(p.cu + p.B), 0), p.T);
-        for (long long t = past + id; t < p.T; t += p.nids) {
+        const int early = min(max(__ldg(p.cu), 0), past);
+        for (long long n = id; n < early + p.T - past; n += p.nids) {
+          const long long t = n < early ? n : past + n - early;
           uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + t * p.Hq * p.D);
           for (int e = lane; e < p.Hq * (p.D >> 3); e += 32) row[e] = make_uint4(0u, 0u, 0u, 0u);
           if (p.lse != nullptr)

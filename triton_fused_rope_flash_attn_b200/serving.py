@@ -38,7 +38,8 @@ def paged_rope_append(q, k, v, k_cache, v_cache, block_table, start_lens, cosp, 
     ``positions[t]`` (``[T]``; -1: not rotated, as a CLS token) where given.
 
     Returns the rotated ``(q, k)``, contiguous, rounded once; ``k_cache`` and
-    ``v_cache`` are written in place.
+    ``v_cache`` are written in place. Tokens outside ``[cu_seqlens[0],
+    cu_seqlens[-1])`` belong to no sequence: neither rotated nor stored.
     """
     q_out, k_out, rc = _ext().paged_append(q, k, v, k_cache, v_cache, block_table, start_lens,
                                            cosp, sinp, cu_seqlens, positions)
@@ -70,8 +71,8 @@ def prompt_attention(q, k, v, cu_seqlens, scale=None, return_lse: bool = False):
     holding the tokens ``[cu_seqlens[b], cu_seqlens[b+1])``; a token sees itself
     and the earlier tokens of its sequence. ``Hq // Hkv`` is at most 128.
     Returns ``o [T, Hq, D]``, with ``return_lse`` also the natural-log row LSE
-    (float32 ``[Hq, T]``). Tokens from ``cu_seqlens[-1]`` on belong to no
-    sequence: output 0, LSE -inf.
+    (float32 ``[Hq, T]``). Tokens outside ``[cu_seqlens[0], cu_seqlens[-1])``
+    belong to no sequence: output 0, LSE -inf.
     """
     o, lse, rc = _ext().prompt(q, k, v, cu_seqlens, scale, return_lse)
     if rc:
