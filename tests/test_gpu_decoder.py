@@ -71,3 +71,38 @@ def test_needs_no_grad():
     with pytest.raises(RuntimeError, match="no_grad"):
         attn.prefill(torch.zeros(5, 256, device="cuda", dtype=torch.bfloat16), [5],
                      PagedKVCache(1, 64, 2, 64))
+
+
+def test_registered_ops_trace_and_agree():
+    """The registered forms give the same bits, pass opcheck, and a compiled step
+    holds them in one graph."""
+    from triton_fused_rope_flash_attn_b200 import (CosSinTable, paged_decode_attention,
+                                                   paged_rope_append, prompt_attention)
+    cs = CosSinTable(100.0, 14, 64, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def rand(*s):
+        return torch.randn(*s, device="cuda", generator=g).bfloat16()
+
+    q, k, v = rand(40, 4, 64), rand(40, 2, 64), rand(40, 2, 64)
+    kc, vc = rand(8, 2, 16, 64), rand(8, 2, 16, 64)
+    table = torch.tensor([[1, 5], [2, 7]], device="cuda", dtype=torch.int32)
+    zero = torch.zeros(2, device="cuda", dtype=torch.int32)
+    cu = torch.tensor([0, 25, 40], device="cuda", dtype=torch.int32)
+    lens = torch.tensor([25, 15], device="cuda", dtype=torch.int32)
+
+    def chain(q, k, v, kc, vc):
+        q, k = torch.ops.frsa.paged_append(q, k, v, kc, vc, table, zero, cs.COSP, cs.SINP, cu)
+        o = torch.ops.frsa.prompt_attn(q, k, v, cu)
+        return o, torch.ops.frsa.paged_decode(q[:2], kc, vc, table, lens)
+
+    kc1, vc1 = kc.clone(), vc.clone()
+    qr, kr = paged_rope_append(q, k, v, kc1, vc1, table, zero, cs.COSP, cs.SINP, cu_seqlens=cu)
+    want = (prompt_attention(qr, kr, v, cu), paged_decode_attention(qr[:2], kc1, vc1, table, lens))
+    kc2, vc2 = kc.clone(), vc.clone()
+    got = torch.compile(chain, fullgraph=True)(q, k, v, kc2, vc2)
+    assert all(torch.equal(a, b) for a, b in zip((*got, kc2, vc2), (*want, kc1, vc1)))
+    torch.library.opcheck(torch.ops.frsa.paged_append.default,
+                          (q, k, v, kc2, vc2, table, zero, cs.COSP, cs.SINP, cu))
+    torch.library.opcheck(torch.ops.frsa.prompt_attn.default, (q, k, v, cu))
+    torch.library.opcheck(torch.ops.frsa.paged_decode.default, (q[:2], kc, vc, table, lens))

@@ -26,12 +26,14 @@
 //   warps 4..11  two softmax warpgroups, one per query tile (thread = row =
 //                TMEM lane)
 //
-// TMEM columns: warpgroup g uses [256 g, 256 g + 128) for the scores, over
-// which it writes P as packed 16-bit pairs, and [256 g + 128, 256 g + 256)
-// for O, which accumulates there over the unit's key tiles. The softmax base
-// is raised (and O rescaled) only when a tile's maximum exceeds it by more
-// than 2^8. P of a tile's first 64 keys is published before the rest is
-// computed. The products of a tile's last keys are cut to the 16-key steps
+// TMEM columns: warpgroup g uses [256 g, 256 g + 128) for the scores and the
+// columns from 256 g + 128 on for O, which accumulates there over the unit's
+// key tiles. P is written as packed 16-bit pairs: for D <= 64 into columns of
+// its own (256 g + 192 on), so that the next scores are computed as soon as
+// these have been read; for larger D over the scores, since TMEM is full. The
+// softmax base is raised (and O rescaled) only when a tile's maximum exceeds
+// it by more than 2^8. P of a tile's first 64 keys is published before the
+// rest is computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
 //
 // What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 513
@@ -75,7 +77,8 @@ struct PromptSmem {
   uint8_t v[KS][NCH][kChunkBytes];
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[KS], k_empty[KS], v_full[KS], v_empty[KS];
-  uint64_t s_full[2], p_full[2][2], o_full[2];   // p_full: [tile][64-key half]
+  // s_free, pv_done at every key tile: NCH == 1 only (else pv_done at a unit's end).
+  uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2];   // p_full: [tile][64-key half]
   uint64_t unit_full[2], unit_empty[2];
   uint64_t next_full;
   alignas(16) uint32_t next[4];   // answer to the request for another unit number
@@ -289,6 +292,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
                   const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
   using Sm = PromptSmem<NCH>;
   constexpr int KS = Sm::KS;
+  constexpr bool kOwnP = NCH == 1;         // P has TMEM columns of its own
+  constexpr uint32_t kPCol = kOwnP ? 192 : 0;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Sm* smp = aligned_smem<Sm>(smem_raw);
   if (smp == nullptr) return;
@@ -307,7 +312,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(&sm.s_full[s], 1);
       mbar_init(&sm.p_full[s][0], 4);
       mbar_init(&sm.p_full[s][1], 4);
-      mbar_init(&sm.o_full[s], 1);
+      mbar_init(&sm.s_free[s], 4);
+      mbar_init(&sm.pv_done[s], 1);
       mbar_init(&sm.unit_full[s], 1);
       mbar_init(&sm.unit_empty[s], 10);   // producer, issuer, eight softmax warps
     }
@@ -460,7 +466,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int ks = ks0 + k;
-            if (ks < ks1) mma_ts_elect(tO, tS + 8 * ks, vd + ks * 128, idO, acc || ks > 0);
+            if (ks < ks1) mma_ts_elect(tO, tS + kPCol + 8 * ks, vd + ks * 128, idO, acc || ks > 0);
           }
         };
         auto last_of = [&](const PromptUnit& y, int g) {
@@ -498,6 +504,12 @@ __global__ void __launch_bounds__(kPrThreads, 1)
             for (int g = 0; g < 2; ++g) {
               if (j >= x.n[g]) continue;
               const int steps = pr_keys(last_of(x, g), j) / 16;
+              const bool more = j + 1 < x.n[g];
+              if (kOwnP && more) {   // the next scores, as soon as these are read
+                mbar_wait(&sm.s_free[g], tg[g] & 1, abort_flag);
+                tc_fence_after();
+                issue_s(g, s1, pr_keys(last_of(x, g), j + 1));
+              }
               mbar_wait(&sm.p_full[g][0], tg[g] & 1, abort_flag);
               tc_fence_after();
               issue_pv(g, s, j > 0, 0, min(steps, 4));
@@ -505,12 +517,9 @@ __global__ void __launch_bounds__(kPrThreads, 1)
               tc_fence_after();
               issue_pv(g, s, true, 4, steps);
               ++tg[g];
-              if (j + 1 == x.n[g]) {
-                mma_commit_elect(&sm.o_full[g]);
-                continue;
-              }
+              if (kOwnP || !more) mma_commit_elect(&sm.pv_done[g]);
               // (in order after the products that read P from the same columns)
-              issue_s(g, s1, pr_keys(last_of(x, g), j + 1));
+              if (!kOwnP && more) issue_s(g, s1, pr_keys(last_of(x, g), j + 1));
               if (j + 2 == x.n[g]) mma_commit_elect(&sm.q_empty[g]);
             }
             mma_commit_elect(&sm.v_empty[s]);
@@ -537,7 +546,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     const int r = wq * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     const float c2 = p.c2;
-    const uint32_t tS = tmem + 256 * g + lane_off, tO = tS + 128;
+    const uint32_t tS = tmem + 256 * g + lane_off, tO = tS + 128, tP = tS + kPCol;
     const int rtok = r / p.G, head = r - rtok * p.G;
     int tg = 0, uo = 0;
     for (int i = 0;; ++i) {
@@ -606,6 +615,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         // The first 64 keys' P with the base so far, then the maximum of the rest;
         // rarely, a new base, and those keys again.
         uint32_t pk0[16], pk1[16];
+        bool pv_waited = j == 0;
 #pragma unroll 1
         for (;;) {
           load(0);
@@ -617,6 +627,12 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           if (64 < keys) {
             load(1);
             mx = fmaxf(mx, half_max());
+          }
+          if (kOwnP && !pv_waited) {   // the products before this tile have read P and written O
+            pv_waited = true;
+            mbar_wait(&sm.pv_done[g], uo & 1, abort_flag);
+            ++uo;
+            tc_fence_after();
           }
           const bool up = mx * c2 > m2 + kPrSlack;
           if (!__any_sync(0xffffffffu, up)) break;
@@ -636,21 +652,26 @@ __global__ void __launch_bounds__(kPrThreads, 1)
             tmem_st16(tO + c16 * 16, w);
           }
         }
-        tmem_st16(tS, pk0);
-        if (32 < keys) tmem_st16(tS + 16, pk1);
+        if (kOwnP) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.s_free[g]);
+        }
+        tmem_st16(tP, pk0);
+        if (32 < keys) tmem_st16(tP + 16, pk1);
         if (64 < keys) exps(0, pk0);   // while the stores complete
         publish(0);
-        if (64 < keys) tmem_st16(tS + 32, pk0);
+        if (64 < keys) tmem_st16(tP + 32, pk0);
         if (96 < keys) {
           exps(1, pk1);
-          tmem_st16(tS + 48, pk1);
+          tmem_st16(tP + 48, pk1);
         }
         publish(1);
         const float2 s0 = f2_get(f2_add(sp[0], sp[1]));
         l += s0.x + s0.y;
       }
       // O / l once the unit's last P V has completed.
-      mbar_wait(&sm.o_full[g], uo & 1, abort_flag);
+      mbar_wait(&sm.pv_done[g], uo & 1, abort_flag);
       ++uo;
       tc_fence_after();
       const bool stored = rtok < p.TT && tok < x.len;
@@ -660,23 +681,23 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       const float inv = 1.f / l;
       bool finite = true;
 #pragma unroll 1
-      for (int c16 = 0; c16 * 16 < DP; ++c16) {
-        float v[16];
-        tmem_ld16(tO + c16 * 16, v);
+      for (int c = 0; c < DP; c += 32) {   // (the last 16 may be past DP: not stored)
+        float v[32];
+        tmem_ld32(tO + c, v);
         tmem_wait_ld();
-        uint4 w[2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          v[e] *= inv;
-          finite &= fabsf(v[e]) < INFINITY;
-        }
-        w[0] = make_uint4(Elt<T>::pack(v[0], v[1]), Elt<T>::pack(v[2], v[3]),
-                          Elt<T>::pack(v[4], v[5]), Elt<T>::pack(v[6], v[7]));
-        w[1] = make_uint4(Elt<T>::pack(v[8], v[9]), Elt<T>::pack(v[10], v[11]),
-                          Elt<T>::pack(v[12], v[13]), Elt<T>::pack(v[14], v[15]));
-        if (stored) {
-          reinterpret_cast<uint4*>(orow)[2 * c16] = w[0];
-          if (c16 * 16 + 8 < p.D) reinterpret_cast<uint4*>(orow)[2 * c16 + 1] = w[1];
+        for (int e = 0; e < 32; e += 8) {
+          if (c + e < p.D) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float y0 = v[e + 2 * k] * inv, y1 = v[e + 2 * k + 1] * inv;
+              finite &= fabsf(y0) < INFINITY && fabsf(y1) < INFINITY;
+              w[k] = Elt<T>::pack(y0, y1);
+            }
+            if (stored)
+              reinterpret_cast<uint4*>(orow + c + e)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
       }
       tc_fence_before();   // O is read before this group's next arrival lets a product overwrite it

@@ -12,6 +12,11 @@ Ops (namespace ``frsa``):
 * ``frsa::attn_fwd(q, k, v, cosp, sinp, has_cls) -> (o, lse)``
 * ``frsa::attn_bwd(q, k, v, o, lse, d_o, cosp, sinp, has_cls) -> (dq, dk, dv)``
 
+* ``frsa::paged_append(q, k, v, k_cache, v_cache, block_table, start_lens, cosp, sinp,
+  cu_seqlens=None, positions=None) -> (q, k)`` (writes the caches)
+* ``frsa::paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale=None) -> o``
+* ``frsa::prompt_attn(q, k, v, cu_seqlens, scale=None) -> o``
+
 ``attn_fwd`` carries an autograd formula that calls ``attn_bwd``.
 ``sdpa_fa_rope_op`` is the differentiable entry with the reference's dtype
 rule (compute in the autocast dtype when autocast is on, outputs in the input
@@ -20,13 +25,14 @@ dtype).
 from __future__ import annotations
 
 import math
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
 
 from .attention import (TritonAttention, _check_tables, _sdpa_comp_dtype,
                         fused_rope_attention_bwd, fused_rope_attention_fwd)
+from .serving import paged_decode_attention, paged_rope_append, prompt_attention
 
 
 @torch.library.custom_op("frsa::attn_fwd", mutates_args=())
@@ -95,3 +101,45 @@ def sdpa_fa_rope_op(Q: Tensor, K: Tensor, V: Tensor, cos_sin, *, has_cls: bool =
     q, k, v = (t.to(comp).contiguous() for t in (Q, K, V))
     o, _ = attn_fwd(q, k, v, COSP.contiguous(), SINP.contiguous(), has_cls)
     return o.to(Q.dtype)
+
+
+# The serving operators: inference only, so without an autograd formula.
+@torch.library.custom_op("frsa::paged_append", mutates_args=("k_cache", "v_cache"))
+def paged_append_op(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor,
+                    block_table: Tensor, start_lens: Tensor, cosp: Tensor, sinp: Tensor,
+                    cu_seqlens: Optional[Tensor] = None,
+                    positions: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """``paged_rope_append``: the rotated ``(q, k)``; the caches are written."""
+    return paged_rope_append(q, k, v, k_cache, v_cache, block_table, start_lens, cosp, sinp,
+                             cu_seqlens=cu_seqlens, positions=positions)
+
+
+@paged_append_op.register_fake
+def _paged_append_fake(q, k, v, k_cache, v_cache, block_table, start_lens, cosp, sinp,
+                       cu_seqlens=None, positions=None):
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+            torch.empty(k.shape, dtype=k.dtype, device=k.device))
+
+
+@torch.library.custom_op("frsa::paged_decode", mutates_args=())
+def paged_decode_op(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
+                    seq_lens: Tensor, scale: Optional[float] = None) -> Tensor:
+    """``paged_decode_attention``."""
+    return paged_decode_attention(q, k_cache, v_cache, block_table, seq_lens, scale)
+
+
+@paged_decode_op.register_fake
+def _paged_decode_fake(q, k_cache, v_cache, block_table, seq_lens, scale=None):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+@torch.library.custom_op("frsa::prompt_attn", mutates_args=())
+def prompt_attn_op(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor,
+                   scale: Optional[float] = None) -> Tensor:
+    """``prompt_attention``."""
+    return prompt_attention(q, k, v, cu_seqlens, scale)
+
+
+@prompt_attn_op.register_fake
+def _prompt_attn_fake(q, k, v, cu_seqlens, scale=None):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
