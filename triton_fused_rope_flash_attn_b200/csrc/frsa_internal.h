@@ -127,6 +127,24 @@ size_t decode_workspace_bytes();
 cudaError_t launch_prompt(const frsa_prompt_args& a, const CUtensorMap& tq, const CUtensorMap& tk,
                           const CUtensorMap& tv, cudaStream_t stream);
 
+// Launch of a kernel that calls wait_previous (frsa_ptx.cuh): its start-up
+// overlaps the end of the kernel before it in the stream.
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem,
+                         cudaStream_t stream, const A&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Number of SMs of the current device (queried once per device).
 int device_sm_count();
 

@@ -83,6 +83,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
   const int per = kAppendThreads / G;         // rows per pass
   const int g = threadIdx.x % G, r0 = threadIdx.x / G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  allow_next();
+  wait_previous();
   const long long t0 = static_cast<long long>(blockIdx.x) * p.tokens;
   const int tokens = static_cast<int>(min(static_cast<long long>(p.tokens), p.T - t0));
 
@@ -426,6 +428,17 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
   const int U = p.Hkv * p.blocks;
   const int grid = gridDim.x, cta = blockIdx.x;
 
+  // Columns past D of the ring are never copied to: zero them.
+  const int pad = 2 * NK - (p.D >> 3);
+  auto zero_pad = [&](int row0, int rows) {
+    for (int i = lane; i < rows * pad; i += 32)
+      *reinterpret_cast<uint4*>(&sm.ring[warp][0][0][0] + (row0 + i / pad) * Sm::kStride +
+                                ((p.D >> 3) + i % pad) * 16) = make_uint4(0u, 0u, 0u, 0u);
+  };
+  if (pad != 0) zero_pad(0, S * 2 * kDecKeys);
+  allow_next();
+  wait_previous();
+
   // Tiles and pieces in all (every warp for itself).
   int total = 0, total_pieces = 0;
   for (int b = lane; b < p.B; b += 32) {
@@ -499,15 +512,6 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
     end = share_begin(cta + 1);
     cur = locate(begin, cur.tile);
   }
-  // Columns past D of the ring are never copied to: zero them.
-  const int pad = 2 * NK - (p.D >> 3);
-  auto zero_pad = [&](int row0, int rows) {
-    for (int i = lane; i < rows * pad; i += 32)
-      *reinterpret_cast<uint4*>(&sm.ring[warp][0][0][0] + (row0 + i / pad) * Sm::kStride +
-                                ((p.D >> 3) + i % pad) * 16) = make_uint4(0u, 0u, 0u, 0u);
-  };
-  if (pad != 0) zero_pad(0, S * 2 * kDecKeys);
-
   // The copying side runs ahead with a cursor of its own. Pages are looked up
   // one tile before their copies: one page for the warp's 16 keys where these
   // cannot straddle two, else lane l (and l + 16) that of key row l & 15. Each
@@ -955,8 +959,7 @@ cudaError_t launch_decode_t(DecodeParams& p, int grid, cudaStream_t stream) {
   const size_t smem = sizeof(DecSmem<NK, NT>);
   const cudaError_t e = set_max_dynamic_smem_once(kern, smem);
   if (e != cudaSuccess) return e;
-  kern<<<grid, kDecThreads, smem, stream>>>(p);
-  return cudaGetLastError();
+  return launch_after(kern, grid, kDecThreads, smem, stream, p);
 }
 
 template <typename T, int NT>
@@ -1021,11 +1024,9 @@ cudaError_t launch_paged_append(const frsa_paged_append_args& a, cudaStream_t st
   // Few tokens: a CTA each, for the shortest chain.
   p.tokens = a.T > 4 * device_sm_count() ? kAppendMost : 1;
   const unsigned grid = static_cast<unsigned>((a.T + p.tokens - 1) / p.tokens);
-  if (a.dtype == FRSA_DTYPE_BF16)
-    paged_append_kernel<__nv_bfloat16><<<grid, kAppendThreads, 0, stream>>>(p);
-  else
-    paged_append_kernel<__half><<<grid, kAppendThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_after(a.dtype == FRSA_DTYPE_BF16 ? paged_append_kernel<__nv_bfloat16>
+                                                 : paged_append_kernel<__half>,
+                      grid, kAppendThreads, 0, stream, p);
 }
 
 cudaError_t launch_paged_decode(const frsa_paged_decode_args& a, cudaStream_t stream) {

@@ -330,6 +330,12 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     tmem_alloc(&sm.tmem_base, 512);
     tmem_relinquish();
   }
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  wait_previous();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -390,9 +396,6 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     } else if (warp == 0) {
       // ---------------------------------------------------------- producer
       if (lane == 0) {
-        tma_prefetch_desc(&tm_q);
-        tma_prefetch_desc(&tm_k);
-        tma_prefetch_desc(&tm_v);
         const uint32_t qbytes = static_cast<uint32_t>(NCH * p.G * p.TT * 128);
         int qf[2] = {0, 0}, kf = 0, vf = 0;   // fills issued
         bool ok = true;
@@ -725,8 +728,7 @@ cudaError_t launch_prompt_t(const PromptParams& p, const CUtensorMap& tq, const 
   auto kern = prompt_kernel<T, NCH>;
   const cudaError_t e = set_max_dynamic_smem_once(kern, smem);
   if (e != cudaSuccess) return e;
-  kern<<<p.nids, kPrThreads, smem, stream>>>(tq, tk, tv, p);
-  return cudaGetLastError();
+  return launch_after(kern, p.nids, kPrThreads, smem, stream, tq, tk, tv, p);
 }
 
 }  // namespace

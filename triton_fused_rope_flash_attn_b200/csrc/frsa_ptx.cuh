@@ -221,6 +221,18 @@ __device__ __forceinline__ bool flag_wait_geq(const int* p, int target, volatile
   }
 }
 
+// ---------------------------------------------------------------- launches
+// A kernel launched by launch_after may start while the one before it in the
+// stream still runs: it waits here, before its first access to global memory,
+// until that one has ended and its writes can be seen. A kernel that calls
+// allow_next lets such a successor start before its own end.
+__device__ __forceinline__ void wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void allow_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- fences
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
