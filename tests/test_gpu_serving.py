@@ -347,6 +347,45 @@ def test_append_index_values_outside():
     assert call([0, 0], positions=ints([39, -1])) == 0
 
 
+# ------------------------------------------------------------------ large offsets
+def test_cache_offsets_past_32_bits():
+    """Pages whose elements lie past 2^32: append and decode there give the bits
+    of a small cache."""
+    g = gen(20)
+    hkv, page, D, n = 8, 64, 128, 150
+    pages = 2 ** 32 // (hkv * page * D) + 8
+    big = [torch.empty(pages, hkv, page, D, device="cuda", dtype=BF) for _ in range(2)]
+    small = [torch.empty(8, hkv, page, D, device="cuda", dtype=BF) for _ in range(2)]
+    cosp, sinp = rope_tables(n + 1, D)
+    q, k, v = (randn(g, n, h, D) for h in (16, hkv, hkv))
+    table = ints([[4, 1, 6]])
+    outs = []
+    for (kc, vc), t in ((small, table), (big, table + (pages - 8))):
+        qr, _ = frsa().paged_rope_append(q, k, v, kc, vc, t, ints([0]), cosp, sinp,
+                                         cu_seqlens=ints([0, n]))
+        outs.append(frsa().paged_decode_attention(qr[-1:], kc, vc, t, ints([n])))
+    assert status() == 0
+    assert torch.equal(outs[0], outs[1])
+    want = decode64(qr[-1:], *small, table, [n], 1 / math.sqrt(D), BF)
+    check(outs[0], want[0], want[1])
+
+
+def test_prompt_offsets_past_31_bits():
+    """More than 2^31 elements of q in 1800 packed sequences: the last ones give
+    the bits of a call of their own."""
+    g = gen(21)
+    n, B, hq, D = 300, 1800, 32, 128
+    T = n * B
+    assert T * hq * D > 2 ** 31
+    q = torch.empty(T, hq, D, device="cuda", dtype=BF).normal_(generator=g)
+    k, v = (torch.empty(T, 1, D, device="cuda", dtype=BF).normal_(generator=g) for _ in range(2))
+    o = frsa().prompt_attention(q, k, v, bounds([n] * B))
+    assert status() == 0
+    for b in (0, 901, B - 1):
+        s = slice(b * n, (b + 1) * n)
+        assert torch.equal(o[s], frsa().prompt_attention(q[s], k[s], v[s], bounds([n])))
+
+
 # ------------------------------------------------------------------ together
 def test_other_streams_and_graphs():
     """The operators run on the current stream; a captured step can be replayed,

@@ -19,8 +19,9 @@ namespace {
 // do not depend on where a token goes, so the first two rows' loads of a
 // thread are issued before the look-ups (sequence, page, table row), a
 // warp's for a token each, whose dependent loads they then overlap. What
-// bounds it: memory for many tokens (one per CTA: 48 us for 8985 tokens of 16
-// + 32 heads of 80, 161 MB; the look-ups' latency counted), the launch for few.
+// bounds it: memory for many tokens (8985 tokens of 16 + 32 heads of 80, 161
+// MB: 36 us, 4.5 TB/s, with one token per CTA 48; 8192 tokens of 32 + 16 heads
+// of 128, 222 MB: 44 us, 5.1 TB/s), the launch for few.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendMost = 4;    // tokens of a CTA at most
 
@@ -216,13 +217,15 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
 //
 // Little work goes otherwise: where all units cut into pieces of up to 4 tiles
 // give no more pieces than CTAs, a CTA has one piece, so short units need no
-// joining.
+// joining. (Pieces of up to 2: three sequences of up to 12987 tokens 22.1
+// against 16.7 us, with more to join; of up to 8: eight sequences of up to
+// 1370 tokens 16.5 against 12.4.)
 //
 // Products: mma m16n8k16 with the keys (S^T = K Q^T) and then the head dim
 // (O^T = V^T P^T) as the 16 rows and 8 query heads as columns, so groups of up
 // to 8 heads fill the columns and the softmax has no padding rows beyond them
-// (against the heads as rows: 521 -> about 200 instructions per warp and
-// tile). P^T moves from the first product's result layout to the second's
+// (with the heads as rows 64 sequences of up to 8000 tokens took 214 us against
+// 194). P^T moves from the first product's result layout to the second's
 // operand layout with movmatrix. The probabilities enter the second product
 // as the sum of two 16-bit values (their rounding and what that left), which
 // keeps them to 2^-16 for bf16.
@@ -240,7 +243,10 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
 // the gain back, in the kernel or in a second one); a fifth warp that copies
 // for all four (a 16-row TMA box takes about 100 cycles: 122 us in all for
 // pages of 16, though 177 against 187 for 64 sequences with pages of 64) or
-// that only schedules.
+// that only schedules. Now 97 us of a call for 131072 tokens (5.5 TB/s), 176 for
+// 64 sequences of up to 8000 tokens (5.9 TB/s, 91 % of the measured copy rate);
+// of 6.0 us for 197 tokens, 2 pass before the first copies (lengths, pages),
+// 1 until they land, 1.5 over four tiles.
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16;                        // keys of a warp in a tile

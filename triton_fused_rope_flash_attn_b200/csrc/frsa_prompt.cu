@@ -36,8 +36,9 @@
 // rest is computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
 //
-// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 513
-// us, 1070 TFLOP/s, 64 % of the card's measured rate. Per 128 keys of a query
+// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 508
+// us, 1080 TFLOP/s, 65 % of the card's measured rate (520 us over longer runs,
+// when the card lowers its clocks under the power limit). Per 128 keys of a query
 // tile 1.5 us of softmax (0.3 of them waits for TMEM, the rest about 700
 // instructions on a chain per row) and 0.4 us of products before the next
 // scores; the two tiles share the SM's exponentials, of which they use half,
