@@ -36,15 +36,18 @@
 // rest is computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
 //
-// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 508
-// us, 1080 TFLOP/s, 65 % of the card's measured rate (520 us over longer runs,
+// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 498
+// us, 1100 TFLOP/s, 66 % of the card's measured rate (more over longer runs,
 // when the card lowers its clocks under the power limit). Per 128 keys of a query
-// tile 1.5 us of softmax (0.3 of them waits for TMEM, the rest about 700
+// tile 1.5 us of softmax (0.3 of them waits for TMEM, the rest about 600
 // instructions on a chain per row) and 0.4 us of products before the next
-// scores; the two tiles share the SM's exponentials, of which they use half,
-// and its tensor core, of which they use half too. Tried and not faster: two
-// threads per row; a fourth or an eighth of the exponentials by a polynomial
-// on the FMA pipe; a thread of its own for each tile's products.
+// scores; the two tiles share the SM's exponentials and its tensor core, of
+// each of which they use 61 %. Tried and not faster: two threads per row; a
+// fourth or an eighth of the exponentials by a polynomial on the FMA pipe; a
+// thread of its own for each tile's products. Not kept: for bf16, whose range
+// would allow it, no maximum per tile but a base raised when the sum has grown
+// (478 us, but a row that rises by more than 2^95 within a tile overflows; with a
+// guard against that 486 us and slower on short prompts).
 //
 // Masked places: keys past a row's position get P = 0, but 0 times an
 // infinity or NaN in V (a later token's, or another sequence's in the same
