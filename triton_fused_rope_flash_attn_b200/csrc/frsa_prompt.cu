@@ -346,11 +346,19 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const uint32_t tmem = sm.tmem_base;
 
   // Unit i of this CTA: slot i & 1 of the unit ring, parity (i >> 1) & 1.
-  // On a wait that gave up the unit counts as the end.
-  auto take_unit = [&](int i) {
+  // On a wait that gave up the unit counts as the end, for all lanes of a warp
+  // alike (take_unit); the producer is a single lane (take_unit_alone).
+  auto take_unit_alone = [&](int i) {
     PromptUnit x;
     x.valid = 0;
     if (mbar_wait(&sm.unit_full[i & 1], (i >> 1) & 1, abort_flag)) x = sm.unit[i & 1];
+    return x;
+  };
+  auto take_unit = [&](int i) {
+    PromptUnit x;
+    x.valid = 0;
+    if (__all_sync(0xffffffffu, mbar_wait(&sm.unit_full[i & 1], (i >> 1) & 1, abort_flag)))
+      x = sm.unit[i & 1];
     return x;
   };
 
@@ -385,9 +393,9 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           mbar_wait(&sm.unit_empty[i & 1], (i >> 1) & 1, abort_flag);
           ++i;
         }
-        if (*abort_flag) break;
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
         if (lane == 0) request_next(sm.next, &sm.next_full);
-        if (!mbar_wait(&sm.next_full, asked & 1, abort_flag)) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.next_full, asked & 1, abort_flag))) {
           mbar_wait_limit(&sm.next_full, asked & 1);   // the answer lands before the CTA ends
           break;
         }
@@ -407,7 +415,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         int qf[2] = {0, 0}, kf = 0, vf = 0;   // fills issued
         bool ok = true;
         for (int i = 0; ok; ++i) {
-          const PromptUnit x = take_unit(i);
+          const PromptUnit x = take_unit_alone(i);
           if (!x.valid) break;
           mbar_arrive(&sm.unit_empty[i & 1]);
           for (int g = 0; g < 2 && ok; ++g) {
