@@ -440,6 +440,35 @@ def test_other_streams_and_graphs():
     assert status() == 0
 
 
+def test_early_started_kernels_see_what_comes_before():
+    """Calls that follow one another without a wait (each may start while the one
+    before it ends) give the bits of calls with the device idle in between:
+    the step's output is the next step's input, and buffers are reused."""
+    g = gen(15)
+    lens = [700, 1, 65]
+    kc0, vc0, table = paged([n + 80 for n in lens], 2, 16, 64, BF, g)
+    cosp, sinp = rope_tables(800, 64)
+    x0 = randn(g, 3, 8, 64)
+    cu = ints([0, 1, 2, 3])
+
+    def chain(wait):
+        kc, vc, n, x = kc0.clone(), vc0.clone(), ints(lens), x0
+        for _ in range(60):
+            q, k = frsa().paged_rope_append(x, x[:, :2], x[:, 2:4], kc, vc, table, n, cosp, sinp)
+            wait()
+            n += 1
+            x = frsa().paged_decode_attention(q, kc, vc, table, n)
+            wait()
+            x = x + frsa().prompt_attention(q, k, x[:, 4:6], cu)
+            wait()
+        return x, kc, vc
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), want))
+    assert status() == 0
+
+
 def test_refusals_on_the_gpu():
     m = frsa()
     g = gen(14)

@@ -53,7 +53,7 @@ __device__ __forceinline__ int find_sequence(const int* cu, int B, long long t, 
   while (n > 1) {
     const int step = (n + 31) / 32;
     const int probe = lo + lane * step;
-    const bool below = lane * step < n && __ldg(cu + probe) <= t;
+    const bool below = lane * step < n && ld_int(cu + probe) <= t;
     const unsigned mask = __ballot_sync(0xffffffffu, below);
     const int i = mask == 0 ? 0 : 31 - __clz(mask);
     n = min(step, n - i * step);
@@ -84,8 +84,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
   const int per = kAppendThreads / G;         // rows per pass
   const int g = threadIdx.x % G, r0 = threadIdx.x / G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  allow_next();
   wait_previous();
+  allow_next();
   const long long t0 = static_cast<long long>(blockIdx.x) * p.tokens;
   const int tokens = static_cast<int>(min(static_cast<long long>(p.tokens), p.T - t0));
 
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
   auto load = [&](const Row& w, uint4(&x)[kAppendMost]) {
 #pragma unroll
     for (int i = 0; i < kAppendMost; ++i)
-      if (i < tokens) x[i] = __ldcs(w.src + i * w.src_step);
+      if (i < tokens) x[i] = ld_stream16(w.src + i * w.src_step);
   };
   // Two rows' loads are in flight.
   const bool works = r0 < per;
@@ -144,18 +144,18 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
     bool held = true;
     if (p.cu_seqlens != nullptr) {
       b = find_sequence(p.cu_seqlens, p.B, t, lane);
-      index = t - __ldg(p.cu_seqlens + b);
-      held = index >= 0 && t < __ldg(p.cu_seqlens + b + 1);
+      index = t - ld_int(p.cu_seqlens + b);
+      held = index >= 0 && t < ld_int(p.cu_seqlens + b + 1);
     }
-    index += __ldg(p.start_lens + b);
-    const long long pos = !held ? -1 : p.positions != nullptr ? __ldg(p.positions + t) : index;
+    index += ld_int(p.start_lens + b);
+    const long long pos = !held ? -1 : p.positions != nullptr ? ld_int(p.positions + t) : index;
     // (in 32 bits: an index past them lies outside every block table)
     const unsigned at = held && index >= 0 && index < (1LL << 31) ? static_cast<unsigned>(index)
                                                                   : 0xffffffffu;
     const unsigned page_no = at / static_cast<unsigned>(p.page_size);
     bool stored = at != 0xffffffffu && page_no < p.max_pages;
     long long page = 0;
-    if (stored) page = __ldg(p.block_table + b * p.bt_stride + page_no);
+    if (stored) page = ld_int(p.block_table + b * p.bt_stride + page_no);
     const bool bad = (held && !stored) || page < 0 || page >= p.num_pages || pos < -1 ||
                      pos >= p.n_pos;
     stored = stored && page >= 0 && page < p.num_pages;
@@ -168,8 +168,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
     const int pairs4 = p.D >> 3;   // float4s of a table row
     float4 f = lane < 16 ? make_float4(1.f, 1.f, 1.f, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
     if (pos >= 0 && pos < p.n_pos && (lane & 15) < pairs4)
-      f = __ldg(reinterpret_cast<const float4*>((lane < 16 ? p.cosp : p.sinp) + pos * (p.D >> 1)) +
-                (lane & 15));
+      f = ld_f4((lane < 16 ? p.cosp : p.sinp) + pos * (p.D >> 1) + (lane & 15) * 4);
     turns[warp][lane >> 4][lane & 15] = f;
   }
   __syncthreads();
@@ -345,7 +344,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 // Cached tokens of sequence b, held within what its block table can name.
 __device__ __forceinline__ int dec_len(const DecodeParams& p, int b) {
-  return min(max(__ldg(p.seq_lens + b), 0), p.max_len);
+  return min(max(ld_int(p.seq_lens + b), 0), p.max_len);
 }
 __device__ __forceinline__ int dec_tiles(int len) { return (len + kDecTile - 1) / kDecTile; }
 __device__ __forceinline__ int dec_pieces(int tiles) { return (tiles + kDecPiece - 1) / kDecPiece; }
@@ -442,8 +441,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
                                 ((p.D >> 3) + i % pad) * 16) = make_uint4(0u, 0u, 0u, 0u);
   };
   if (pad != 0) zero_pad(0, S * 2 * kDecKeys);
-  allow_next();
   wait_previous();
+  allow_next();
 
   // Tiles and pieces in all (every warp for itself).
   int total = 0, total_pieces = 0;
@@ -463,7 +462,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
   // Sequences with nothing cached: zero output, lse -inf.
   auto empty_sequences = [&]() {
     for (int b = cta; b < p.B; b += grid) {
-      const int n = __ldg(p.seq_lens + b);
+      const int n = ld_int(p.seq_lens + b);
       if (n > 0 && n <= p.max_len) continue;
       if (n != 0 && threadIdx.x == 0) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
       if (n > 0) continue;
@@ -542,7 +541,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
     w.head_off = ahead.h * p.head_g;
     if (key < ahead.len) {
       const int pi = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-      w.page = __ldg(p.block_table + ahead.b * p.bt_stride + pi);
+      w.page = ld_int(p.block_table + ahead.b * p.bt_stride + pi);
       w.slot = key - pi * p.page_size;
     }
     return w;
@@ -654,8 +653,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
           for (int i = 0; i < 2; ++i) {
             const int row = nt * 8 + quad, col = ks * 16 + i * 8 + ql * 2;
             qb[nt][ks][i] = (row < rows && col < p.D)
-                                ? __ldg(reinterpret_cast<const uint32_t*>(
-                                      qp + cur.b * p.qs[0] + (h0 + row) * p.qs[1] + col))
+                                ? ld_u32(qp + cur.b * p.qs[0] + (h0 + row) * p.qs[1] + col)
                                 : 0u;
           }
 #pragma unroll

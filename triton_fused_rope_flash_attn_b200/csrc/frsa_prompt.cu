@@ -107,7 +107,7 @@ struct PromptParams {
 
 // Tokens [start, end) of sequence b, held within [0, T).
 __device__ __forceinline__ void pr_sequence(const PromptParams& p, int b, int& start, int& len) {
-  const int s = __ldg(p.cu + b), e = __ldg(p.cu + b + 1);
+  const int s = ld_int(p.cu + b), e = ld_int(p.cu + b + 1);
   start = min(max(s, 0), p.T);
   len = max(min(e, p.T) - start, 0);
   if (s < 0 || e < s || e > p.T) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
@@ -267,7 +267,7 @@ __device__ __noinline__ void slow_row(const PromptParams& p, long long tq, int h
     float s = 0.f;
 #pragma unroll 1
     for (int d = 0; d < pairs; ++d) {
-      const float2 a = Elt<T>::unpack(__ldg(qr + d)), b = Elt<T>::unpack(__ldg(kr + d));
+      const float2 a = Elt<T>::unpack(qr[d]), b = Elt<T>::unpack(kr[d]);
       s = fmaf(a.x, b.x, fmaf(a.y, b.y, s));
     }
     s *= p.c2;
@@ -278,7 +278,7 @@ __device__ __noinline__ void slow_row(const PromptParams& p, long long tq, int h
     l = l * alpha + w;
 #pragma unroll 1
     for (int d = 0; d < pairs; ++d) {
-      const float2 x = Elt<T>::unpack(__ldg(vr + d));
+      const float2 x = Elt<T>::unpack(vr[d]);
       acc[2 * d] = acc[2 * d] * alpha + w * x.x;
       acc[2 * d + 1] = acc[2 * d + 1] * alpha + w * x.y;
     }
@@ -371,8 +371,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         const PromptUnit x = pr_find_unit(p, id, lane);
         // Tokens before the first sequence and after the last belong to none:
         // zero output.
-        const int past = min(max(__ldg(p.cu + p.B), 0), p.T);
-        const int early = min(max(__ldg(p.cu), 0), past);
+        const int past = min(max(ld_int(p.cu + p.B), 0), p.T);
+        const int early = min(max(ld_int(p.cu), 0), past);
         for (long long n = id; n < early + p.T - past; n += p.nids) {
           const long long t = n < early ? n : past + n - early;
           uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + t * p.Hq * p.D);

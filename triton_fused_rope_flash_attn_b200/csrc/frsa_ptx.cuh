@@ -225,12 +225,39 @@ __device__ __forceinline__ bool flag_wait_geq(const int* p, int target, volatile
 // A kernel launched by launch_after may start while the one before it in the
 // stream still runs: it waits here, before its first access to global memory,
 // until that one has ended and its writes can be seen. A kernel that calls
-// allow_next lets such a successor start before its own end.
+// allow_next, after its own wait, lets such a successor start before its own
+// end. Loads behind the wait are volatile or ordinary ones: __ldg and its like
+// are no memory accesses to the compiler, which may move them up past the wait,
+// and are meant for data that does not change while the kernel runs.
 __device__ __forceinline__ void wait_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 __device__ __forceinline__ void allow_next() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ int ld_int(const int* p) {
+  int v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_u32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 ld_f4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_stream16(const void* p) {   // read once
+  uint4 v;
+  asm volatile("ld.global.cs.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
 // ---------------------------------------------------------------- fences
