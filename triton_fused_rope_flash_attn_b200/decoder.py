@@ -70,7 +70,10 @@ class PagedKVCache:
     def advance(self, new) -> None:
         """Count ``new[b]`` appended tokens of each sequence."""
         self.host_lens = [n + m for n, m in zip(self.host_lens, new)]
-        self.lens.copy_(torch.tensor(self.host_lens, dtype=torch.int32))
+        if len(set(new)) == 1:   # a step: no copy from the host
+            self.lens += new[0]
+        else:
+            self.lens.copy_(torch.tensor(self.host_lens, dtype=torch.int32))
 
     def release(self, b: int) -> None:
         """Sequence ``b`` is done: its pages are free again."""
