@@ -493,6 +493,9 @@ def test_refusals_on_the_gpu():
     raises(RuntimeError, randn(g, 1, 4, 60), *(randn(g, 4, 2, 16, 60) for _ in range(2)), table, n)
     raises(RuntimeError, randn(g, 1, 4, 136), *(randn(g, 4, 2, 16, 136) for _ in range(2)), table, n)
     raises(RuntimeError, q, *(randn(g, 4, 2, 16, 68)[..., :64] for _ in range(2)), table, n)
+    for scale in (0.0, -1.0, math.nan):
+        raises(ValueError, q, kc, vc, table, n, scale=scale)
+        raises(ValueError, q, k, k, ints([0, 1]), scale=scale, fn=m.prompt_attention)
     raises(RuntimeError, q.clone().requires_grad_(), kc, vc, table, n)
     with torch.no_grad():
         m.paged_decode_attention(q.clone().requires_grad_(), kc, vc, table, n)
