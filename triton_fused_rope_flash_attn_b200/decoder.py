@@ -7,8 +7,9 @@ rotation and tables, but causal, with fewer kv heads than query heads if
 wanted, prompts of different lengths packed without padding, and one new token
 per sequence and step:
 
-    cache = PagedKVCache(batch=2, max_len=256, num_kv_heads=4, head_dim=64)
-    attn = CausalRopeAttention(1024, 16, 4, CosSinTable(100.0, 14, 64))
+    rope = CosSinTable(100.0, 16, 64)   # 256 positions: a CLS token and 256 patches
+    cache = PagedKVCache(batch=2, max_len=257, num_kv_heads=4, head_dim=64)
+    attn = CausalRopeAttention(1024, 16, 4, rope, device="cuda", dtype=torch.bfloat16)
     with torch.no_grad():
         y = attn.prefill(x, [197, 60], cache)     # x [257, 1024]: the prompts' tokens
         y = attn.step(x_new, cache)               # x_new [2, 1024]: a token each
@@ -88,8 +89,8 @@ class CausalRopeAttention(nn.Module):
 
     ``rope`` is any module with ``tables()`` (``CosSinTable`` for patches in
     raster order); token ``i`` of a sequence is rotated with table row ``i -
-    has_cls``, the CLS token not at all. Inference only: call it under
-    ``torch.no_grad()``.
+    has_cls``, the CLS token not at all. A token whose row the table does not
+    have is refused. Inference only: call it under ``torch.no_grad()``.
     """
 
     def __init__(self, dim: int, num_heads: int, num_kv_heads: int, rope, has_cls: bool = True,
@@ -109,12 +110,22 @@ class CausalRopeAttention(nn.Module):
         qkv = self.qkv(x).view(x.shape[0], -1, self.head_dim)
         return qkv.split((self.num_heads, self.num_kv_heads, self.num_kv_heads), dim=1)
 
+    def _tables(self, new, cache: PagedKVCache):
+        """The rotation tables, which have to reach ``new[b]`` more tokens of each sequence."""
+        cosp, sinp = self.rope.tables()
+        for b, (have, n) in enumerate(zip(cache.host_lens, new)):
+            if n and have + n - int(self.has_cls) > cosp.shape[0]:
+                raise ValueError(f"sequence {b}: {have + n} tokens, the rotation table has "
+                                 f"{cosp.shape[0]} positions")
+        return cosp, sinp
+
     def prefill(self, x: torch.Tensor, lens, cache: PagedKVCache) -> torch.Tensor:
         """Whole prompts, ``x [sum(lens), dim]``, one per sequence of the (empty) cache."""
         if any(cache.host_lens):
             raise ValueError("prefill starts from an empty cache")
         if x.shape[0] != sum(lens):
             raise ValueError(f"{x.shape[0]} tokens for prompts of {sum(lens)}")
+        tables = self._tables(lens, cache)
         cache.reserve(lens)
         q, k, v = self._project(x)
         bounds, index = [0], []
@@ -123,7 +134,7 @@ class CausalRopeAttention(nn.Module):
             index.append(torch.arange(n, dtype=torch.int32) - int(self.has_cls))
         cu = torch.tensor(bounds, dtype=torch.int32).to(x.device)
         q, k = paged_rope_append(q, k, v, cache.k, cache.v, cache.block_table, cache.lens,
-                                 *self.rope.tables(), cu_seqlens=cu,
+                                 *tables, cu_seqlens=cu,
                                  positions=torch.cat(index).to(x.device))
         cache.advance(lens)
         o = prompt_attention(q, k, v, cu)
@@ -132,10 +143,11 @@ class CausalRopeAttention(nn.Module):
     def step(self, x: torch.Tensor, cache: PagedKVCache) -> torch.Tensor:
         """One new token of every sequence, ``x [batch, dim]``."""
         one = [1] * x.shape[0]
+        tables = self._tables(one, cache)
         cache.reserve(one)
         q, k, v = self._project(x)
         q, _ = paged_rope_append(q, k, v, cache.k, cache.v, cache.block_table, cache.lens,
-                                 *self.rope.tables(),
+                                 *tables,
                                  positions=cache.lens - 1 if self.has_cls else None)
         cache.advance(one)
         o = paged_decode_attention(q, cache.k, cache.v, cache.block_table, cache.lens)
