@@ -6,6 +6,7 @@
 // [i * page_size, (i + 1) * page_size) of sequence b.
 #include "frsa_internal.h"
 #include "frsa_ptx.cuh"
+#include "frsa_row.cuh"
 
 namespace frsa {
 
@@ -227,7 +228,10 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
 // 194). P^T moves from the first product's result layout to the second's
 // operand layout with movmatrix. The probabilities enter the second product
 // as the sum of two 16-bit values (their rounding and what that left), which
-// keeps them to 2^-16 for bf16.
+// keeps them to 2^-16 for bf16. What was left is zero or negative for some, so
+// an infinity in V, which by the definition makes its column infinite, comes
+// out of that product as NaN. A row that is written with a NaN which no NaN in
+// its V explains is therefore computed again in f32 (dec_mend).
 //
 // A unit within one share is written at once. For the others each share leaves
 // its (m, l, o) in the workspace, and the last of the unit's CTAs to arrive (a
@@ -418,6 +422,39 @@ __device__ __forceinline__ void cp_async_wait_to(int pending) {
     if (pending == N) cp_async_wait<N>();
     else cp_async_wait_to<N - 1>(pending);
   }
+}
+
+// The keys of one (sequence, kv head) for frsa_row.cuh.
+struct DecKeys {
+  const uint4* kc;
+  const uint4* vc;
+  const int* table;    // the sequence's row of the block table
+  long long head_off;
+  uint32_t page_g, slot_g;
+  int page_size, num_pages;
+  int n, granules;
+  __device__ const uint4* row(const uint4* cache, int j) const {
+    const int pi = j / page_size, page = ld_int(table + pi);
+    if (page < 0 || page >= num_pages) return nullptr;
+    return cache + static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_g +
+           static_cast<uint64_t>(static_cast<uint32_t>(j - pi * page_size)) * slot_g + head_off;
+  }
+  __device__ const uint4* k(int j) const { return row(kc, j); }
+  __device__ const uint4* v(int j) const { return row(vc, j); }
+};
+
+// Row (cur.b, head) as it was written, by a whole warp: where it holds a NaN
+// that no NaN in its V explains, it is computed again. Costs about 25
+// instructions per key and warp, only there.
+template <typename T>
+__device__ __noinline__ void dec_mend(const DecKeys& keys, const T* q, float c2, float m, float l,
+                                      T* orow) {
+  const int g = threadIdx.x & 15;
+  uint32_t want = 0;
+  if (g < keys.granules) want = nan_bits<T>(reinterpret_cast<const uint4*>(orow)[g]);
+  if (!__any_sync(kWholeWarp, want != 0)) return;
+  const uint32_t left = want & ~nan_columns<T>(keys, keys.n, want);
+  if (__any_sync(kWholeWarp, left != 0)) exact_row<T>(keys, q, c2, dec_base(m), l, orow);
 }
 
 template <typename T, int NK, int NT>
@@ -922,6 +959,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
       __syncthreads();   // sm.last is read
     }
     if (write) {
+      bool odd = false;   // a NaN that does not come from the row's scores
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float inv[2] = {1.f / l[nt][0], 1.f / l[nt][1]};
@@ -930,6 +968,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
           const int ks = warp + j * kDecWarps;
           if (ks >= NK) continue;
           const float(&v)[4] = acc[nt][j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) odd |= isnan(v[i]) && l[nt][i & 1] > 0.f;
           // Back from O^T: head quad, columns 2 ql, + 1 (and + 8).
           const uint32_t w0 = transpose8x8(Elt<T>::pack(v[0] * inv[0], v[1] * inv[1]));
           const uint32_t w1 = transpose8x8(Elt<T>::pack(v[2] * inv[0], v[3] * inv[1]));
@@ -944,6 +984,27 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
           p.lse[row0 + nt * 8 + ql * 2 + quad] =
               ((quad == 0 ? m[nt][0] : m[nt][1]) + log2f(quad == 0 ? l[nt][0] : l[nt][1])) *
               0.69314718055994531f;
+      }
+      if (__syncthreads_or(odd)) {   // (the barrier orders the rows' writes before their reads)
+        const DecKeys keys = {kc, vc, p.block_table + cur.b * p.bt_stride, cur.h * p.head_g,
+                              p.page_g, p.slot_g, p.page_size, p.num_pages, cur.len, p.D >> 3};
+#pragma unroll 1
+        for (int r = warp; r < rows; r += kDecWarps) {
+          float mr = 0.f, lr = 0.f;   // head r: lane (r & 7) / 2, column r & 1 of part r / 8
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float a = __shfl_sync(kWholeWarp, m[nt][c], (r & 7) >> 1);
+              const float b = __shfl_sync(kWholeWarp, l[nt][c], (r & 7) >> 1);
+              if (nt == r >> 3 && c == (r & 1)) mr = a, lr = b;
+            }
+          if (lr > 0.f)
+            dec_mend<T>(keys,
+                        qp + cur.b * p.qs[0] +
+                            (cur.h * p.group + cur.blk * 8 * NT + r) * p.qs[1],
+                        p.c2, mr, lr, static_cast<T*>(p.o) + (row0 + r) * p.D);
+        }
       }
     }
     fresh = true;
