@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from serving_ref import check, check_lse, decode64, paged
+from serving_ref import U, check, check_lse, decode64, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,71 @@ def test_decode_infinity_of_small_weight():
         o = frsa().paged_decode_attention(q, kc, vc, table, ints([n]), scale=1.0)
         assert (o[0, :, 9] == -math.inf).all()
         assert int(torch.isfinite(o).sum()) == 2 * (D - 1)
+
+
+# ------------------------------------------------------------------ f16: small probabilities
+def tail_rows(n, tail, D):
+    """q, k, v of one head in f16: token 0 scores 0 and has v = 0, every other one
+    scores -tail and has a v of about one."""
+    q, k = (torch.zeros(n, 1, D, device="cuda", dtype=HF) for _ in range(2))
+    q[..., 0] = 1.0
+    k[1:, :, 0] = -tail
+    v = 1.0 + 0.25 * torch.rand(n, 1, D, device="cuda", generator=gen(n), dtype=torch.float32)
+    v[0] = 0.0
+    return q, k, v.to(HF)
+
+
+def tail_tol(o, A, V, n, D, floor, u):
+    """Relative to the largest probability a held one is off by u of itself or by
+    half a step at `floor`, and counts |v|; the rest as in serving_ref. (The score
+    is one product, so exact but for the rounding of its base-2 form: 18 nats
+    times 2^-23.)"""
+    return U[HF] * o.abs() + 2.0 ** -25 + (u + 2 * 18 * 2.0 ** -23 + n * 2.0 ** -24 +
+                                           2.0 ** -20) * A + floor * V
+
+
+@pytest.mark.parametrize("n", [300, 4096, 131072])
+@pytest.mark.parametrize("tail", [14.0, 16.0, 17.0, 17.40625, 18.0])
+def test_f16_decode_keeps_small_probabilities(n, tail):
+    """An attention sink over a long cache: what lies far below the largest
+    probability is all of the output. Two parts of 2^-11 each carry 2^-22 of a
+    probability; f16's smallest half step is 2^-25, at least 2^14 below which the
+    largest probability has to lie: floor 2^-39."""
+    D, page = 64, 16
+    q, k, v = tail_rows(n, tail, D)
+    kc, vc, table = paged([n], 1, page, D, HF, gen(2))
+    at = torch.arange(n, device="cuda")
+    kc[table[0, at // page].long(), :, at % page] = k
+    vc[table[0, at // page].long(), :, at % page] = v
+    o, lse = frsa().paged_decode_attention(q[:1], kc, vc, table, ints([n]), scale=1.0,
+                                           return_lse=True)
+    w = math.exp(-tail)
+    V = v[:, 0].double().sum(0)
+    want = V * w / (1 + (n - 1) * w)
+    tol = tail_tol(want, want, V, n, D, 2.0 ** -39, 2.0 ** -22)
+    check(o[0, 0], want, tol, "o")
+    check(lse[0], torch.full((1,), math.log1p((n - 1) * w), dtype=torch.float64, device="cuda"),
+          torch.full((1,), 2.0 ** -19 + n * 2.0 ** -24 * n * w, dtype=torch.float64, device="cuda"))
+
+
+def big_scores(D, dtype):
+    """Scores of 2^27 and more that rise by 2^17 from key to key: each row is its
+    last key's v alone, and a probability's rounding of 2^4 (half a step of the
+    score's base-2 form) must not take it out of f16's range."""
+    n = 1000
+    q, k = (torch.zeros(n, 1, D, device="cuda", dtype=dtype) for _ in range(2))
+    q[..., 0] = 2.0 ** 13
+    k[:, 0, 0] = 2.0 ** 14 + 16 * torch.arange(n, device="cuda")
+    return q, k, randn(gen(D), n, 1, D, dtype=dtype)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_f16_decode_large_scores(D):
+    q, k, v = big_scores(D, HF)
+    kc, vc, table = paged([1000], 1, 8, D, HF, gen(2))
+    at = torch.arange(1000, device="cuda")
+    kc[table[0, at // 8].long(), :, at % 8] = k
+    vc[table[0, at // 8].long(), :, at % 8] = v
+    for n in (1, 100, 1000):
+        o = frsa().paged_decode_attention(q[:1], kc, vc, table, ints([n]), scale=1.0)
+        assert torch.equal(o[0, 0], v[n - 1, 0])

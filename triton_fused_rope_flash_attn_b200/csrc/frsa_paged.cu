@@ -228,7 +228,11 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
 // 194). P^T moves from the first product's result layout to the second's
 // operand layout with movmatrix. The probabilities enter the second product
 // as the sum of two 16-bit values (their rounding and what that left), which
-// keeps them to 2^-16 for bf16. What was left is zero or negative for some, so
+// keeps them to 2^-16 for bf16 and 2^-22 for f16. f16's smallest step, 2^-24,
+// would be coarse beside probabilities far below the largest one (an attention
+// sink: with the tail 17 nats below it 44 % of the output), so there the
+// softmax base lies kDecLift below the maximum and the largest probability is
+// 2^15; a part's rounding is then at most 2^-40 of it. What was left is zero or negative for some, so
 // an infinity in V, which by the definition makes its column infinite, comes
 // out of that product as NaN. A row that is written with a NaN which no NaN in
 // its V explains is therefore computed again in f32 (dec_mend).
@@ -409,6 +413,10 @@ __device__ __forceinline__ int dec_find(const DecodeParams& p, bool by_piece, in
   }
   return lo;
 }
+
+// log2 of the largest probability that a warp forms: f16's largest power of two.
+template <typename T>
+constexpr float kDecLift = Elt<T>::kBf16 ? 0.f : 15.f;
 
 // exp2 base of a running maximum (a row whose scores are all -inf has none).
 __device__ __forceinline__ float dec_base(float m) { return m == -INFINITY ? 0.f : m; }
@@ -670,7 +678,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
 
   uint32_t qb[NT][NK][2];
   float o[NT][NK][4];   // O^T: rows 16 ks + quad, + 8; columns (heads) 8 nt + 2 ql, + 1
-  float m[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2];   // m: the base, kDecLift below the maximum
   bool fresh = true;
   const T* qp = static_cast<const T*>(p.q);
   const uint32_t ka = ring0 + ((lane >> 3 & 1) * 8 + (lane & 7)) * Sm::kStride + (lane >> 4) * 16;
@@ -736,6 +744,10 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
         for (int d = 4; d < 32; d <<= 1) {
           mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
           mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
+        }
+        if constexpr (!Elt<T>::kBf16) {   // rounded up: no probability passes 2^15
+          mx[0] = __fsub_ru(mx[0], kDecLift<T>);
+          mx[1] = __fsub_ru(mx[1], kDecLift<T>);
         }
         // Earlier sums move to the new base where a maximum rose.
         if (__any_sync(0xffffffffu, mx[0] > m[nt][0] || mx[1] > m[nt][1])) {
