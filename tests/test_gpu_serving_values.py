@@ -157,3 +157,40 @@ def test_f16_decode_large_scores(D):
     for n in (1, 100, 1000):
         o = frsa().paged_decode_attention(q[:1], kc, vc, table, ints([n]), scale=1.0)
         assert torch.equal(o[0, 0], v[n - 1, 0])
+
+
+@pytest.mark.parametrize("n,D,at", [(300, 64, 0), (4096, 64, 0), (4096, 128, 0), (4096, 80, 1500)])
+@pytest.mark.parametrize("tail", [14.0, 16.0, 17.0, 17.40625, 18.0])
+def test_f16_prompt_keeps_small_probabilities(n, D, at, tail):
+    """The same in a prompt, with the large score first or in the middle. One part
+    of a probability carries 2^-11 of it; with the largest one at 2^11 or above
+    f16's smallest half step is a floor of 2^-36."""
+    q, k, v = tail_rows(n, tail, D)
+    k[0], k[at] = k[at].clone(), k[0].clone()
+    v[0], v[at] = v[at].clone(), v[0].clone()
+    o, lse = frsa().prompt_attention(q, k, v, bounds([n]), scale=1.0, return_lse=True)
+    assert status() == 0
+    x = k[:, 0, 0].double()
+    p = torch.exp(x)
+    V = v[:, 0].double().cumsum(0)
+    l = p.cumsum(0)[:, None]
+    want = (p[:, None] * v[:, 0].double()).cumsum(0) / l
+    # rows before the large score: probabilities relative to the largest of the row
+    top = torch.cummax(x, 0).values.exp()[:, None]
+    tol = tail_tol(want, want, V * top / l, n, D, 2.0 ** -36, 2.0 ** -11)
+    check(o[:, 0], want, tol, "o")
+    check(lse[0], l[:, 0].log(), torch.full((n,), 2.0 ** -18 + n * 2.0 ** -23, dtype=torch.float64,
+                                            device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_large_scores(D, dtype):
+    q, k, v = big_scores(D, dtype)
+    if dtype == BF:   # 2^14 + 16 j in steps of 2^7
+        k, v = k[::16], v[::16]
+        q = q[:k.shape[0]]
+    k[:, 0, 0] = k[:, 0, 0].sort().values
+    o = frsa().prompt_attention(q, k, v, bounds([k.shape[0]]), scale=1.0)
+    assert k[:, 0, 0].double().diff().min() >= 16
+    assert status() == 0 and torch.equal(o[:, 0], v[:, 0])

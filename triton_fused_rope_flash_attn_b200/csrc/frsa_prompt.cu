@@ -31,8 +31,8 @@
 // key tiles. P is written as packed 16-bit pairs: for D <= 64 into columns of
 // its own (256 g + 192 on), so that the next scores are computed as soon as
 // these have been read; for larger D over the scores, since TMEM is full. The
-// softmax base is raised (and O rescaled) only when a tile's maximum exceeds
-// it by more than 2^8. P of a tile's first 64 keys is published before the
+// softmax base is raised (and O rescaled) only when a tile's maximum leaves
+// the range above it (PrBase). P of a tile's first 64 keys is published before the
 // rest is computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
 //
@@ -63,7 +63,23 @@ namespace {
 constexpr int kPrThreads = 384;
 // Registers per thread after the split (launch: 168 each; 88 + 2 x 208 = 3 x 168).
 constexpr uint32_t kPrRegsCtl = 88, kPrRegsSoftmax = 208;
-constexpr float kPrSlack = 8.f;   // log2 headroom of the softmax base
+// Softmax base (log2): set kLift below a maximum, raised when a tile's maximum
+// lies more than kRange above it. The sums and O, in f32, do not mind; P is
+// rounded to the type and has to stay in its range. bf16: the most headroom
+// that was measured. f16, whose smallest step is 2^-24: P of a row's largest
+// score lies between 2^11 and 2^15, so that what lies 2^-25 below it (17 nats)
+// is still normal and the rounding of smaller ones at most 2^-36 of it. (With
+// the base at the maximum a tail 17 nats below one large score was 40 % off.)
+template <typename T>
+struct PrBase {
+  static constexpr float kLift = Elt<T>::kBf16 ? 0.f : 11.f;
+  static constexpr float kRange = Elt<T>::kBf16 ? 8.f : 15.f;
+  // The base's own step passes 8 at 2^27, and then P may leave f16's range: such
+  // a row is computed again in f32.
+  static __device__ bool coarse(float base) {
+    return !Elt<T>::kBf16 && fabsf(base) >= 134217728.f;
+  }
+};
 
 struct PromptUnit {
   int valid;       // 0: no more units
@@ -563,7 +579,9 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    using Base = PrBase<T>;
     const float c2 = p.c2;
+    auto base_of = [&](float mx) { return __fmaf_ru(mx, c2, -Base::kLift); };
     const uint32_t tS = tmem + 256 * g + lane_off, tO = tS + 128, tP = tS + kPCol;
     const int rtok = r / p.G, head = r - rtok * p.G;
     int tg = 0, uo = 0;
@@ -638,7 +656,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         for (;;) {
           load(0);
           float mx = half_max();
-          if (m2 == -INFINITY) m2 = mx * c2;   // (the unit's first tile)
+          // (Bases are rounded up, so that no exponent passes kRange.)
+          if (m2 == -INFINITY) m2 = base_of(mx);   // (the unit's first tile)
           sp[0] = sp[1] = f2_make(0.f, 0.f);
           exps(0, pk0);
           exps(1, pk1);
@@ -652,9 +671,9 @@ __global__ void __launch_bounds__(kPrThreads, 1)
             ++uo;
             tc_fence_after();
           }
-          const bool up = mx * c2 > m2 + kPrSlack;
+          const bool up = __fmaf_ru(mx, c2, -m2) > Base::kRange;
           if (!__any_sync(0xffffffffu, up)) break;
-          const float mn = up ? mx * c2 : m2;
+          const float mn = up ? base_of(mx) : m2;
           const float alpha = ex2(m2 - mn);
           l *= alpha;
           m2 = mn;
@@ -722,7 +741,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       if (stored) {
         float* ls = p.lse == nullptr ? nullptr : p.lse + static_cast<long long>(h) * p.T + tq;
         if (ls != nullptr) *ls = (m2 + log2f(l)) * 0.69314718055994531f;
-        if (!finite) slow_row<T>(p, tq, h, x.kvh, x.start, tok + 1, orow, ls);
+        if (!finite || Base::coarse(m2)) slow_row<T>(p, tq, h, x.kvh, x.start, tok + 1, orow, ls);
       }
       __syncwarp();
     }
