@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from serving_ref import U, check, check_lse, decode64, paged
+from serving_ref import U, check, check_lse, decode64, paged, prompt64
 
 pytestmark = pytest.mark.gpu
 
@@ -194,3 +194,167 @@ def test_prompt_large_scores(D, dtype):
     o = frsa().prompt_attention(q, k, v, bounds([k.shape[0]]), scale=1.0)
     assert k[:, 0, 0].double().diff().min() >= 16
     assert status() == 0 and torch.equal(o[:, 0], v[:, 0])
+
+
+# ------------------------------------------------------------------ prompt: values that are not finite
+def fastest_ms(fn, runs=7):
+    fn()
+    best = math.inf
+    for _ in range(runs):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        torch.cuda.synchronize()
+        a.record()
+        fn()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF), (64, HF), (128, BF), (128, HF)])
+def test_prompt_nan_early_in_a_long_prompt(D, dtype):
+    """One NaN in the first token of 8192: the result where it is not seen and where
+    it is, no status, and about the time of a call without it (all rows behind it
+    hold a NaN that is theirs)."""
+    n, hq, hkv = 8192, 4, 2
+    g = gen(D)
+    q, k, v = (randn(g, n, h, D, dtype=dtype) for h in (hq, hkv, hkv))
+    cu = bounds([n])
+    want = prompt64(q, k, v, [n], 1 / math.sqrt(D), dtype)
+    clean = fastest_ms(lambda: frsa().prompt_attention(q, k, v, cu))
+    for what in ("element", "row", "key"):
+        k2, v2 = k.clone(), v.clone()
+        hit = torch.zeros(n, hq, D, dtype=torch.bool, device="cuda")
+        if what == "element":
+            v2[0, 1, 7] = math.nan
+            hit[:, 2:, 7] = True
+        elif what == "row":
+            v2[0, 1] = math.nan
+            hit[:, 2:] = True
+        else:
+            k2[0, 1] = math.nan
+            hit[:, 2:] = True
+        o, lse = frsa().prompt_attention(q, k2, v2, cu, return_lse=True)
+        assert status() == 0
+        assert torch.isnan(o[hit]).all()
+        check(o[~hit], want[0][~hit], want[1][~hit], what)
+        if what == "key":
+            assert torch.isnan(lse[2:]).all()
+            check_lse(lse[:2], want[2][:2], want[3][:2])
+        else:
+            check_lse(lse, want[2], want[3])
+        ms = fastest_ms(lambda: frsa().prompt_attention(q, k2, v2, cu))
+        assert ms < 3 * clean + 0.1, f"{what}: {ms:.3f} ms, without {clean:.3f}"
+
+
+@pytest.mark.parametrize("hq,hkv,D,dtype", [(2, 2, 64, BF), (8, 2, 128, HF), (12, 4, 80, BF),
+                                            (3, 1, 72, HF), (16, 1, 128, BF)])
+def test_prompt_masked_values_beside_visible_ones(hq, hkv, D, dtype):
+    """Early tokens with an infinity or NaN that later rows see, and later tokens
+    with others that earlier rows of the same tiles must not see; the last token
+    of one sequence and the first of the next."""
+    g = gen(hq * D)
+    lens = [300, 41, 200]
+    cu = bounds(lens)
+    q, k, v = (randn(g, 541, h, D, dtype=dtype) for h in (hq, hkv, hkv))
+    want = prompt64(q, k, v, lens, 1 / math.sqrt(D), dtype)
+    v2 = v.clone()
+    col = torch.zeros(541, hkv, D, dtype=torch.float64, device="cuda")   # what rows get instead
+    ends = [300, 341, 541]
+    for t, x, c in ((10, math.inf, 3), (130, math.nan, 3), (131, math.nan, 5), (200, -math.inf, 9),
+                    (299, math.nan, 0), (300, math.inf, 1), (340, -math.inf, D - 1),
+                    (341, math.nan, 0), (540, math.inf, 2)):
+        v2[t, 0, c] = x
+        end = min(e for e in ends if e > t)
+        col[t:end, 0, c] += x
+    o = frsa().prompt_attention(q, k, v2, cu).double()
+    assert status() == 0
+    put = col.repeat_interleave(hq // hkv, 1)
+    hit = put != 0
+    assert torch.equal(torch.isnan(o[hit]), torch.isnan(put[hit]))
+    same = hit & ~torch.isnan(put)
+    assert torch.equal(o[same], put[same])
+    check(o[~hit], want[0][~hit], want[1][~hit])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_infinity_of_small_weight(D):
+    """An infinity 60 nats below the largest score is seen all the same, in f16 too,
+    whose rounded probability there is 0."""
+    for dtype in (BF, HF):
+        n = 3000
+        q, k = (torch.zeros(n, 1, D, device="cuda", dtype=dtype) for _ in range(2))
+        q[..., 0] = 1.0
+        k[0, 0, 0] = 60.0
+        v = randn(gen(D), n, 1, D, dtype=dtype)
+        v[100, 0, 9] = -math.inf
+        o = frsa().prompt_attention(q, k, v, bounds([n]), scale=1.0)
+        assert status() == 0
+        assert (o[100:, 0, 9] == -math.inf).all()
+        assert int(torch.isfinite(o).sum()) == n * D - (n - 100)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, BF), (64, HF), (80, HF)])
+def test_prompt_scores_of_minus_infinity(D, dtype):
+    """Keys whose score is -inf count nothing, also where they fill whole tiles
+    before the first other one; rows that see nothing else have lse -inf."""
+    n = 700
+    g = gen(D)
+    for holes in ([(0, 200)], [(0, 64), (100, 500)], [(0, 128)], [(0, 400), (401, 650)]):
+        q, k, v = (randn(g, n, h, D, dtype=dtype) for h in (2, 1, 1))
+        q[..., 0] = 1.0
+        k[..., 0] = 0.0
+        out = torch.zeros(n, dtype=torch.bool, device="cuda")
+        for a, b in holes:
+            k[a:b, 0, 0] = -math.inf
+            out[a:b] = True
+        o, lse = frsa().prompt_attention(q, k, v, bounds([n]), return_lse=True)
+        assert status() == 0
+        first = int((~out).nonzero()[0])
+        k2 = k.clone()
+        k2[out] = 0
+        from serving_ref import attend64
+        mask = torch.ones(n, n, dtype=torch.bool, device="cuda").tril() & ~out
+        want = attend64(q.transpose(0, 1), k2.transpose(0, 1).repeat_interleave(2, 0),
+                        v.transpose(0, 1).repeat_interleave(2, 0), 1 / math.sqrt(D), mask, dtype,
+                        False)
+        check(o.transpose(0, 1)[:, first:], want[0][:, first:], want[1][:, first:])
+        check_lse(lse, want[2], want[3])
+
+
+def test_prompt_large_values():
+    """v near the end of bf16's range, a score that rises by 2^7.9 within the first
+    tile: the sum over probabilities of at most 1 stays in f32's range."""
+    for D in (64, 128):
+        n = 128
+        q, k = (torch.zeros(n, 1, D, device="cuda", dtype=BF) for _ in range(2))
+        q[..., 0] = 1.0
+        k[64:, 0, 0] = 7.875 * math.log(2.0)
+        v = torch.full((n, 1, D), 2.0 ** 120, device="cuda", dtype=BF)
+        o = frsa().prompt_attention(q, k, v, bounds([n]), scale=1.0)
+        assert status() == 0
+        assert ((o.double() / 2.0 ** 120 - 1).abs() <= 2.0 ** -8 + 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [10, 24, 40, 59])
+def test_prompt_scores_far_past_their_step(D, power):
+    """bf16 scores of 2^(2 power): every row is the v of its largest score, the last
+    key's, which is twice the one before it (and so on, eight times over)."""
+    n = 200
+    q, k = (torch.zeros(n, 1, D, device="cuda", dtype=BF) for _ in range(2))
+    q[..., 0] = 2.0 ** power
+    for lens in ([n], [1] * n, [8] * 25):
+        first = [0]
+        for m in lens:
+            first.append(first[-1] + m)
+        j = torch.cat([torch.arange(m) for m in lens]).cuda()
+        k[:, 0, 0] = 2.0 ** (power - 8 + (j % 8).float()) * (1 + (j // 8).float() / 128)
+        v = randn(gen(D), n, 1, D)
+        o, lse = frsa().prompt_attention(q, k, v, bounds(lens), scale=1.0, return_lse=True)
+        assert status() == 0
+        s = (q[:, 0, 0].double() * k[:, 0, 0].double())
+        for a, b in zip(first[:-1], first[1:]):
+            top, at = torch.cummax(s[a:b], 0)
+            assert torch.equal(o[a:b, 0], v[a:b, 0][at])
+            assert ((lse[0, a:b].double() - top).abs() <= top.abs() * 2.0 ** -22).all()

@@ -452,17 +452,16 @@ struct DecKeys {
 };
 
 // Row (cur.b, head) as it was written, by a whole warp: where it holds a NaN
-// that no NaN in its V explains, it is computed again. Costs about 25
+// that no NaN in its V explains, it is computed again. Costs about 30
 // instructions per key and warp, only there.
 template <typename T>
-__device__ __noinline__ void dec_mend(const DecKeys& keys, const T* q, float c2, float m, float l,
-                                      T* orow) {
+__device__ __noinline__ void dec_mend(const DecKeys& keys, const T* q, float c2, T* orow) {
   const int g = threadIdx.x & 15;
   uint32_t want = 0;
   if (g < keys.granules) want = nan_bits<T>(reinterpret_cast<const uint4*>(orow)[g]);
   if (!__any_sync(kWholeWarp, want != 0)) return;
   const uint32_t left = want & ~nan_columns<T>(keys, keys.n, want);
-  if (__any_sync(kWholeWarp, left != 0)) exact_row<T>(keys, q, c2, dec_base(m), l, orow);
+  if (__any_sync(kWholeWarp, left != 0)) exact_row<T>(keys, q, c2, orow);
 }
 
 template <typename T, int NK, int NT>
@@ -1002,20 +1001,19 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm)
                               p.page_g, p.slot_g, p.page_size, p.num_pages, cur.len, p.D >> 3};
 #pragma unroll 1
         for (int r = warp; r < rows; r += kDecWarps) {
-          float mr = 0.f, lr = 0.f;   // head r: lane (r & 7) / 2, column r & 1 of part r / 8
+          bool sound = false;   // l of head r: lane (r & 7) / 2, column r & 1 of part r / 8
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const float a = __shfl_sync(kWholeWarp, m[nt][c], (r & 7) >> 1);
-              const float b = __shfl_sync(kWholeWarp, l[nt][c], (r & 7) >> 1);
-              if (nt == r >> 3 && c == (r & 1)) mr = a, lr = b;
-            }
-          if (lr > 0.f)
+            for (int c = 0; c < 2; ++c)
+              if (__shfl_sync(kWholeWarp, l[nt][c], (r & 7) >> 1) > 0.f && nt == r >> 3 &&
+                  c == (r & 1))
+                sound = true;
+          if (sound)
             dec_mend<T>(keys,
                         qp + cur.b * p.qs[0] +
                             (cur.h * p.group + cur.blk * 8 * NT + r) * p.qs[1],
-                        p.c2, mr, lr, static_cast<T*>(p.o) + (row0 + r) * p.D);
+                        p.c2, static_cast<T*>(p.o) + (row0 + r) * p.D);
         }
       }
     }

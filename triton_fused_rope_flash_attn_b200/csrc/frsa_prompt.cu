@@ -23,6 +23,10 @@
 //                next one that has not started (clusterlaunchcontrol), so the
 //                longest units, which come first, are shared out as SMs get
 //                free
+//   warp 3       mender: rows that hold a NaN (below). It has a warp of its own
+//                because the same code in the softmax warps, inlined or called,
+//                costs them 3 % where there is nothing to mend (one prompt of 8192
+//                tokens 507 against 484 us)
 //   warps 4..11  two softmax warpgroups, one per query tile (thread = row =
 //                TMEM lane)
 //
@@ -51,10 +55,17 @@
 //
 // Masked places: keys past a row's position get P = 0, but 0 times an
 // infinity or NaN in V (a later token's, or another sequence's in the same
-// tile) would still reach O. A row whose result is not finite is therefore
-// computed again on its own, from its visible keys alone (slow_row).
+// tile) would still reach O. It makes NaN, so a row that holds a NaN is looked
+// at again (pr_mend): where NaN in the V of keys that it sees explain it, that
+// is the result; otherwise the row is computed once more in f32, from its keys
+// alone (exact_row). One NaN early in a sequence thus costs the rows behind it a
+// search that ends with the key that holds it. What is computed again are the rows
+// of the tiles at the masked value, and in f16 rows whose P rounds to 0 at an
+// infinity: about 30 instructions a key and row. The limit of the waits applies to
+// the time between two rows then.
 #include "frsa_internal.h"
 #include "frsa_ptx.cuh"
+#include "frsa_row.cuh"
 
 namespace frsa {
 
@@ -65,21 +76,25 @@ constexpr int kPrThreads = 384;
 constexpr uint32_t kPrRegsCtl = 88, kPrRegsSoftmax = 208;
 // Softmax base (log2): set kLift below a maximum, raised when a tile's maximum
 // lies more than kRange above it. The sums and O, in f32, do not mind; P is
-// rounded to the type and has to stay in its range. bf16: the most headroom
-// that was measured. f16, whose smallest step is 2^-24: P of a row's largest
+// rounded to the type and has to stay in its range. bf16 has f32's: P between
+// 2^-8 and 1 for a row's largest score, so that O stays in range where the result
+// does. f16, whose smallest step is 2^-24: P of a row's largest
 // score lies between 2^11 and 2^15, so that what lies 2^-25 below it (17 nats)
 // is still normal and the rounding of smaller ones at most 2^-36 of it. (With
 // the base at the maximum a tail 17 nats below one large score was 40 % off.)
 template <typename T>
 struct PrBase {
-  static constexpr float kLift = Elt<T>::kBf16 ? 0.f : 11.f;
-  static constexpr float kRange = Elt<T>::kBf16 ? 8.f : 15.f;
-  // The base's own step passes 8 at 2^27, and then P may leave f16's range: such
-  // a row is computed again in f32.
-  static __device__ bool coarse(float base) {
-    return !Elt<T>::kBf16 && fabsf(base) >= 134217728.f;
-  }
+  static constexpr float kLift = Elt<T>::kBf16 ? -8.f : 11.f;
+  static constexpr float kRange = Elt<T>::kBf16 ? 0.f : 15.f;
+  // From here on the base's own step, by which it may lie above the scores, takes
+  // P out of the range (f16: 16 at 2^27; bf16: 64 at 2^29): such a row is computed
+  // again in f32.
+  static constexpr float kCoarse = Elt<T>::kBf16 ? 536870912.f : 134217728.f;
 };
+
+// Base of a row with no score above -inf so far: finite, so that such scores give
+// P = 0, and below every other.
+constexpr float kPrNone = -3e38f;
 
 struct PromptUnit {
   int valid;       // 0: no more units
@@ -87,6 +102,14 @@ struct PromptUnit {
   int tok0;        // first token (in the sequence) of query tile 0; tile 1 follows at + TT
   int kvh;
   int n[2];        // key tiles of each query tile (0: the tile has no tokens)
+};
+
+// What a softmax warp asks the mender to look at: rows (bits) of a query tile that
+// begins at token t0 of the sequence from token `start` on; odd: the row holds a
+// NaN, redo: it is computed again in any case.
+struct Mend {
+  int start, kvh, t0;
+  unsigned odd, redo;
 };
 
 template <int NCH>
@@ -101,10 +124,14 @@ struct PromptSmem {
   uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2];   // p_full: [tile][64-key half]
   uint64_t unit_full[2], unit_empty[2];
   uint64_t next_full;
+  uint64_t mend_full[2], mend_empty[2];
   alignas(16) uint32_t next[4];   // answer to the request for another unit number
   PromptUnit unit[2];
+  Mend mend[2][8];
+  int mend_end[2];
   uint32_t tmem_base;
   int abort_flag;
+  uint32_t beat;   // rows that the mender has looked at
 };
 
 struct PromptParams {
@@ -263,47 +290,68 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// One query row from global memory, in f32, over its visible keys only.
+// The keys of one (sequence, kv head) for frsa_row.cuh.
+struct PrKeys {
+  const uint4* k0;
+  const uint4* v0;
+  long long ks, vs;   // token strides in granules
+  int n, granules;
+  __device__ const uint4* k(int j) const { return k0 + j * ks; }
+  __device__ const uint4* v(int j) const { return v0 + j * vs; }
+};
+
+// The 32 rows from `row0` on of a query tile, as they were written, by a whole warp.
 template <typename T>
-__device__ __noinline__ void slow_row(const PromptParams& p, long long tq, int h, int kvh,
-                                      long long key0, int nkeys, T* orow, float* lse) {
-  const T* q = static_cast<const T*>(p.q) + tq * p.qs[0] + h * p.qs[1];
-  const T* k = static_cast<const T*>(p.k) + key0 * p.ks[0] + kvh * p.ks[1];
-  const T* v = static_cast<const T*>(p.v) + key0 * p.vs[0] + kvh * p.vs[1];
-  float acc[128];
-  const int pairs = p.D / 2;
-#pragma unroll 1
-  for (int d = 0; d < p.D; ++d) acc[d] = 0.f;
-  float m = -INFINITY, l = 0.f;
-#pragma unroll 1
-  for (int j = 0; j < nkeys; ++j) {
-    const uint32_t* kr = reinterpret_cast<const uint32_t*>(k + j * p.ks[0]);
-    const uint32_t* vr = reinterpret_cast<const uint32_t*>(v + j * p.vs[0]);
-    const uint32_t* qr = reinterpret_cast<const uint32_t*>(q);
-    float s = 0.f;
-#pragma unroll 1
-    for (int d = 0; d < pairs; ++d) {
-      const float2 a = Elt<T>::unpack(qr[d]), b = Elt<T>::unpack(kr[d]);
-      s = fmaf(a.x, b.x, fmaf(a.y, b.y, s));
-    }
-    s *= p.c2;
-    const float mn = fmaxf(m, s);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = ex2(m - base), w = ex2(s - base);
-    m = mn;
-    l = l * alpha + w;
-#pragma unroll 1
-    for (int d = 0; d < pairs; ++d) {
-      const float2 x = Elt<T>::unpack(vr[d]);
-      acc[2 * d] = acc[2 * d] * alpha + w * x.x;
-      acc[2 * d + 1] = acc[2 * d + 1] * alpha + w * x.y;
-    }
+__device__ __forceinline__ void pr_mend(const PromptParams& p, const Mend& a, int row0,
+                                        volatile uint32_t* beat) {
+  const int lane = threadIdx.x & 31;
+  const bool odd = a.odd >> lane & 1;
+  PrKeys keys;
+  keys.k0 = reinterpret_cast<const uint4*>(static_cast<const T*>(p.k) + a.start * p.ks[0] +
+                                           a.kvh * p.ks[1]);
+  keys.v0 = reinterpret_cast<const uint4*>(static_cast<const T*>(p.v) + a.start * p.vs[0] +
+                                           a.kvh * p.vs[1]);
+  keys.ks = p.ks[0] >> 3;
+  keys.vs = p.vs[0] >> 3;
+  keys.granules = p.D >> 3;
+  auto token = [&](int r) { return a.t0 + r / p.G; };
+  auto head = [&](int r) { return a.kvh * p.G + r % p.G; };
+  auto out = [&](int r) {
+    return static_cast<T*>(p.o) + (static_cast<long long>(a.start + token(r)) * p.Hq + head(r)) * p.D;
+  };
+  if (lane == 0) *beat = *beat + 1;
+  // NaN columns of the lane's row (8 bits a granule) and, at lane & 15 = granule,
+  // of all rows.
+  uint32_t mine[4] = {0u, 0u, 0u, 0u}, want = 0;
+#pragma unroll
+  for (int g = 0; g < 16; ++g) {
+    if (g >= keys.granules) break;
+    const uint32_t bits =
+        odd ? nan_bits<T>(reinterpret_cast<const uint4*>(out(row0 + lane))[g]) : 0u;
+    mine[g >> 2] |= bits << (8 * (g & 3));
+    const uint32_t all = __reduce_or_sync(kWholeWarp, bits);
+    if ((lane & 15) == g) want = all;
   }
-  const float inv = 1.f / l;
-#pragma unroll 1
-  for (int d = 0; d < pairs; ++d)
-    reinterpret_cast<uint32_t*>(orow)[d] = Elt<T>::pack(acc[2 * d] * inv, acc[2 * d + 1] * inv);
-  if (lse != nullptr) *lse = (m + log2f(l)) * 0.69314718055994531f;
+  // The keys that the first row sees all rows see.
+  const uint32_t seen = __any_sync(kWholeWarp, want != 0)
+                            ? nan_columns<T>(keys, __shfl_sync(kWholeWarp, token(row0) + 1, 0), want)
+                            : 0u;
+  bool again = a.redo >> lane & 1;
+#pragma unroll
+  for (int g = 0; g < 16; ++g)
+    again |= (mine[g >> 2] >> (8 * (g & 3)) & 0xffu & ~__shfl_sync(kWholeWarp, seen, g)) != 0;
+  unsigned todo = __ballot_sync(kWholeWarp, again);
+  while (todo != 0) {
+    const int i = __ffs(todo) - 1, r = row0 + i;
+    todo &= todo - 1;
+    if (lane == 0) *beat = *beat + 1;
+    keys.n = __shfl_sync(kWholeWarp, token(r) + 1, 0);
+    const float lse = exact_row<T>(
+        keys, static_cast<const T*>(p.q) + (a.start + token(r)) * p.qs[0] + head(r) * p.qs[1],
+        p.c2, out(r));
+    if (p.lse != nullptr && lane == i)
+      p.lse[static_cast<long long>(head(r)) * p.T + a.start + token(r)] = lse;
+  }
 }
 
 template <typename T, int NCH>
@@ -323,9 +371,13 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const int lane = threadIdx.x & 31;
   const int DP = (p.D + 15) & ~15;
   volatile int* abort_flag = &sm.abort_flag;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity, abort_flag, &sm.beat);
+  };
 
   if (threadIdx.x == 0) {
     sm.abort_flag = 0;
+    sm.beat = 0;
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sm.q_full[s], 1);
       mbar_init(&sm.q_empty[s], 1);
@@ -336,6 +388,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(&sm.pv_done[s], 1);
       mbar_init(&sm.unit_full[s], 1);
       mbar_init(&sm.unit_empty[s], 10);   // producer, issuer, eight softmax warps
+      mbar_init(&sm.mend_full[s], 8);
+      mbar_init(&sm.mend_empty[s], 1);
     }
     for (int s = 0; s < KS; ++s) {
       mbar_init(&sm.k_full[s], 1);
@@ -344,6 +398,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(&sm.v_empty[s], 1);
     }
     mbar_init(&sm.next_full, 1);
+    sm.mend_end[0] = sm.mend_end[1] = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -367,13 +422,13 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   auto take_unit_alone = [&](int i) {
     PromptUnit x;
     x.valid = 0;
-    if (mbar_wait(&sm.unit_full[i & 1], (i >> 1) & 1, abort_flag)) x = sm.unit[i & 1];
+    if (wait(&sm.unit_full[i & 1], (i >> 1) & 1)) x = sm.unit[i & 1];
     return x;
   };
   auto take_unit = [&](int i) {
     PromptUnit x;
     x.valid = 0;
-    if (__all_sync(0xffffffffu, mbar_wait(&sm.unit_full[i & 1], (i >> 1) & 1, abort_flag)))
+    if (__all_sync(0xffffffffu, wait(&sm.unit_full[i & 1], (i >> 1) & 1)))
       x = sm.unit[i & 1];
     return x;
   };
@@ -406,12 +461,12 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           // Another unit is asked for when this one's softmax begins. (Three
           // ahead, CTAs were done between 391 and 439 us of one prompt of 8192
           // tokens.)
-          mbar_wait(&sm.unit_empty[i & 1], (i >> 1) & 1, abort_flag);
+          wait(&sm.unit_empty[i & 1], (i >> 1) & 1);
           ++i;
         }
         if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
         if (lane == 0) request_next(sm.next, &sm.next_full);
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.next_full, asked & 1, abort_flag))) {
+        if (!__all_sync(0xffffffffu, wait(&sm.next_full, asked & 1))) {
           mbar_wait_limit(&sm.next_full, asked & 1);   // the answer lands before the CTA ends
           break;
         }
@@ -436,7 +491,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           mbar_arrive(&sm.unit_empty[i & 1]);
           for (int g = 0; g < 2 && ok; ++g) {
             if (x.n[g] == 0) continue;
-            if (!(ok = mbar_wait(&sm.q_empty[g], (qf[g] & 1) ^ 1, abort_flag))) break;
+            if (!(ok = wait(&sm.q_empty[g], (qf[g] & 1) ^ 1))) break;
             mbar_arrive_expect_tx(&sm.q_full[g], qbytes);
             for (int c = 0; c < NCH; ++c)
               tma_load_3d(sm.q[g][c], &tm_q, &sm.q_full[g], c * kChunkCols, x.kvh * p.G,
@@ -446,14 +501,14 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           const int nmax = max(x.n[0], x.n[1]);
           for (int j = 0; j < nmax && ok; ++j) {
             int s = kf % KS;
-            if (!(ok = mbar_wait(&sm.k_empty[s], ((kf / KS) & 1) ^ 1, abort_flag))) break;
+            if (!(ok = wait(&sm.k_empty[s], ((kf / KS) & 1) ^ 1))) break;
             mbar_arrive_expect_tx(&sm.k_full[s], NCH * kChunkBytes);
             for (int c = 0; c < NCH; ++c)
               tma_load_3d(sm.k[s][c], &tm_k, &sm.k_full[s], c * kChunkCols, x.kvh,
                           x.start + j * kTile);
             ++kf;
             s = vf % KS;
-            if (!(ok = mbar_wait(&sm.v_empty[s], ((vf / KS) & 1) ^ 1, abort_flag))) break;
+            if (!(ok = wait(&sm.v_empty[s], ((vf / KS) & 1) ^ 1))) break;
             mbar_arrive_expect_tx(&sm.v_full[s], NCH * kChunkBytes);
             for (int c = 0; c < NCH; ++c)
               tma_load_3d(sm.v[s][c], &tm_v, &sm.v_full[s], c * kChunkCols, x.kvh,
@@ -469,6 +524,21 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           if (kf >= b) mbar_wait_limit(&sm.k_full[(kf - b) % KS], ((kf - b) / KS) & 1);
           if (vf >= b) mbar_wait_limit(&sm.v_full[(vf - b) % KS], ((vf - b) / KS) & 1);
         }
+      }
+    } else if (warp == 3) {
+      // ------------------------------------------------------------ mender
+      for (int i = 0;; ++i) {
+        const int s = i & 1;
+        if (!__all_sync(kWholeWarp, wait(&sm.mend_full[s], (i >> 1) & 1))) break;
+        if (sm.mend_end[s]) break;
+#pragma unroll 1
+        for (int w = 0; w < 8; ++w) {
+          const Mend a = sm.mend[s][w];
+          if ((a.odd | a.redo) != 0)
+            pr_mend<T>(p, a, (w & 3) * 32, &sm.beat);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.mend_empty[s]);
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
@@ -511,10 +581,10 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         // A unit's scores against its first key tile (tile number `tile`).
         auto first_scores = [&](const PromptUnit& y, int tile) {
           const int s = tile % KS;
-          mbar_wait(&sm.k_full[s], (tile / KS) & 1, abort_flag);
+          wait(&sm.k_full[s], (tile / KS) & 1);
           for (int g = 0; g < 2; ++g) {
             if (y.n[g] == 0) continue;
-            mbar_wait(&sm.q_full[g], qf[g] & 1, abort_flag);
+            wait(&sm.q_full[g], qf[g] & 1);
             ++qf[g];
             tc_fence_after();
             issue_s(g, s, pr_keys(last_of(y, g), 0));
@@ -533,21 +603,21 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           y.valid = 0;
           for (int j = 0; j < nmax; ++j, ++t) {
             const int s = t % KS, s1 = (t + 1) % KS;
-            mbar_wait(&sm.v_full[s], (t / KS) & 1, abort_flag);
-            if (j + 1 < nmax) mbar_wait(&sm.k_full[s1], ((t + 1) / KS) & 1, abort_flag);
+            wait(&sm.v_full[s], (t / KS) & 1);
+            if (j + 1 < nmax) wait(&sm.k_full[s1], ((t + 1) / KS) & 1);
             for (int g = 0; g < 2; ++g) {
               if (j >= x.n[g]) continue;
               const int steps = pr_keys(last_of(x, g), j) / 16;
               const bool more = j + 1 < x.n[g];
               if (kOwnP && more) {   // the next scores, as soon as these are read
-                mbar_wait(&sm.s_free[g], tg[g] & 1, abort_flag);
+                wait(&sm.s_free[g], tg[g] & 1);
                 tc_fence_after();
                 issue_s(g, s1, pr_keys(last_of(x, g), j + 1));
               }
-              mbar_wait(&sm.p_full[g][0], tg[g] & 1, abort_flag);
+              wait(&sm.p_full[g][0], tg[g] & 1);
               tc_fence_after();
               issue_pv(g, s, j > 0, 0, min(steps, 4));
-              mbar_wait(&sm.p_full[g][1], tg[g] & 1, abort_flag);
+              wait(&sm.p_full[g][1], tg[g] & 1);
               tc_fence_after();
               issue_pv(g, s, true, 4, steps);
               ++tg[g];
@@ -585,21 +655,38 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     const uint32_t tS = tmem + 256 * g + lane_off, tO = tS + 128, tP = tS + kPCol;
     const int rtok = r / p.G, head = r - rtok * p.G;
     int tg = 0, uo = 0;
+    // What the mender has to look at in unit i (of every unit: it waits for all
+    // eight warps).
+    auto tell = [&](int i, const Mend& a, int end) {
+      wait(&sm.mend_empty[i & 1], ((i >> 1) & 1) ^ 1);
+      if (lane == 0) {
+        sm.mend[i & 1][warp - 4] = a;
+        if (end) sm.mend_end[i & 1] = 1;
+      }
+      __syncwarp();   // (orders the warp's rows before the mender's reads)
+      if (lane == 0) mbar_arrive(&sm.mend_full[i & 1]);
+    };
     for (int i = 0;; ++i) {
       const PromptUnit x = take_unit(i);
-      if (!x.valid) break;
+      if (!x.valid) {
+        tell(i, Mend{0, 0, 0, 0u, 0u}, 1);
+        break;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.unit_empty[i & 1]);
-      if (x.n[g] == 0) continue;
+      if (x.n[g] == 0) {
+        tell(i, Mend{0, 0, 0, 0u, 0u}, 0);
+        continue;
+      }
       const int t0 = x.tok0 + g * p.TT;
       const int tok = t0 + rtok;
       const int last = min(x.len, t0 + p.TT);
       const int see = min(tok, last - 1);   // the last key this row sees
-      float m2 = -INFINITY, l = 0.f;
+      float m2 = kPrNone, l = 0.f;
       for (int j = 0; j < x.n[g]; ++j, ++tg) {
         const int keys = pr_keys(last, j);
         const bool edge = j * kTile + kTile - 1 > t0;   // some row does not see all keys
-        mbar_wait(&sm.s_full[g], tg & 1, abort_flag);
+        wait(&sm.s_full[g], tg & 1);
         tc_fence_after();
         const int lim = see - j * kTile;   // the last key of the tile that this row sees
         // 64 scores at a time: with 96 or 128 in registers the compiler has none
@@ -657,7 +744,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           load(0);
           float mx = half_max();
           // (Bases are rounded up, so that no exponent passes kRange.)
-          if (m2 == -INFINITY) m2 = base_of(mx);   // (the unit's first tile)
+          if (m2 == kPrNone) m2 = fmaxf(base_of(mx), kPrNone);   // (the unit's first tile)
           sp[0] = sp[1] = f2_make(0.f, 0.f);
           exps(0, pk0);
           exps(1, pk1);
@@ -667,7 +754,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           }
           if (kOwnP && !pv_waited) {   // the products before this tile have read P and written O
             pv_waited = true;
-            mbar_wait(&sm.pv_done[g], uo & 1, abort_flag);
+            wait(&sm.pv_done[g], uo & 1);
             ++uo;
             tc_fence_after();
           }
@@ -708,7 +795,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         l += s0.x + s0.y;
       }
       // O / l once the unit's last P V has completed.
-      mbar_wait(&sm.pv_done[g], uo & 1, abort_flag);
+      wait(&sm.pv_done[g], uo & 1);
       ++uo;
       tc_fence_after();
       const bool stored = rtok < p.TT && tok < x.len;
@@ -716,7 +803,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       const long long tq = x.start + tok;
       T* orow = static_cast<T*>(p.o) + (tq * p.Hq + h) * p.D;
       const float inv = 1.f / l;
-      bool finite = true;
+      bool odd = false;   // a NaN in O
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {   // (the last 16 may be past DP: not stored)
         float v[32];
@@ -729,7 +816,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float y0 = v[e + 2 * k] * inv, y1 = v[e + 2 * k + 1] * inv;
-              finite &= fabsf(y0) < INFINITY && fabsf(y1) < INFINITY;
+              odd |= isnan(v[e + 2 * k]) || isnan(v[e + 2 * k + 1]);
               w[k] = Elt<T>::pack(y0, y1);
             }
             if (stored)
@@ -738,12 +825,14 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         }
       }
       tc_fence_before();   // O is read before this group's next arrival lets a product overwrite it
-      if (stored) {
-        float* ls = p.lse == nullptr ? nullptr : p.lse + static_cast<long long>(h) * p.T + tq;
-        if (ls != nullptr) *ls = (m2 + log2f(l)) * 0.69314718055994531f;
-        if (!finite || Base::coarse(m2)) slow_row<T>(p, tq, h, x.kvh, x.start, tok + 1, orow, ls);
-      }
-      __syncwarp();
+      if (stored && p.lse != nullptr)
+        p.lse[static_cast<long long>(h) * p.T + tq] = (m2 + log2f(l)) * 0.69314718055994531f;
+      // (l is NaN where a score is, and there is no base where all scores are -inf:
+      // the row is NaN then.)
+      const bool redo = stored && l >= 0.f && m2 > kPrNone && fabsf(m2) >= Base::kCoarse;
+      const bool look = stored && l > 0.f && odd;
+      tell(i, Mend{x.start, x.kvh, t0, __ballot_sync(kWholeWarp, look),
+                   __ballot_sync(kWholeWarp, redo)}, 0);
     }
   }
 

@@ -137,11 +137,12 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Wait until the phase with the given parity has completed. Returns false (and
-// leaves the CTA in abort mode) if the wait timed out (FRSA_WAIT_LIMIT_NS) or
-// the CTA was already aborting. The loop is one short PTX block so that the
-// many wait sites of a kernel stay small in the instruction cache.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// Wait until the phase with the given parity has completed. Returns false if the
+// wait timed out (FRSA_WAIT_LIMIT_NS) or the CTA was already aborting. The loop
+// is one short PTX block so that the many wait sites of a kernel stay small in
+// the instruction cache.
+__device__ __forceinline__ bool mbar_wait_once(uint64_t* bar, uint32_t parity,
+                                               volatile int* abort_flag) {
   uint32_t ok;
   asm volatile(
       "{\n\t"
@@ -170,11 +171,32 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
       : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(abort_flag))),
         "l"(static_cast<uint64_t>(FRSA_WAIT_LIMIT_NS))
       : "memory");
-  if (ok) return true;
+  return ok != 0;
+}
+
+// The same; a wait that timed out leaves the CTA in abort mode.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_wait_once(bar, parity, abort_flag)) return true;
   if (*abort_flag == 0) {   // this wait timed out (not an abort raised elsewhere)
     *abort_flag = 1;
     atomicExch(&g_dev_status, FRSA_DEV_TIMEOUT);
   }
+  return false;
+}
+
+// The same behind work that may take longer than the limit: `beat` counts its
+// steps, and the limit is one on the time without a step.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                          const volatile uint32_t* beat) {
+  for (uint32_t seen = 0;;) {
+    if (mbar_wait_once(bar, parity, abort_flag)) return true;
+    const uint32_t now = *beat;
+    if (*abort_flag != 0) return false;
+    if (now == seen) break;
+    seen = now;
+  }
+  *abort_flag = 1;
+  atomicExch(&g_dev_status, FRSA_DEV_TIMEOUT);
   return false;
 }
 
