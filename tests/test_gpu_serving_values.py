@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from serving_ref import U, check, check_lse, decode64, paged, prompt64
+from serving_ref import U, check, check_lse, decode64, paged, prompt64, rope_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -358,3 +358,59 @@ def test_prompt_scores_far_past_their_step(D, power):
             top, at = torch.cummax(s[a:b], 0)
             assert torch.equal(o[a:b, 0], v[a:b, 0][at])
             assert ((lse[0, a:b].double() - top).abs() <= top.abs() * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("hq,hkv,D,dtype", [(4, 2, 64, HF), (2, 1, 128, BF)])
+def test_prompt_many_values_that_are_not_finite(hq, hkv, D, dtype):
+    """One element of v in a hundred is not finite: nearly every row has masked ones
+    in its last tile, and each column is what its visible values make it."""
+    n = 3000
+    g = gen(D)
+    q, k, v = (randn(g, n, h, D, dtype=dtype) for h in (hq, hkv, hkv))
+    want = prompt64(q, k, v, [n], 1 / math.sqrt(D), dtype)
+    u = torch.rand(n, hkv, D, device="cuda", generator=g)
+    u[:1000, :, 3:] = 1.0     # (first only three columns, so that others stay finite)
+    u[:, :, D // 2:] = 1.0
+    v[u < 0.01] = math.inf
+    v[(u >= 0.01) & (u < 0.015)] = -math.inf
+    v[(u >= 0.015) & (u < 0.016)] = math.nan
+    put = torch.where(torch.isfinite(v.double()), 0.0, v.double()).cumsum(0)
+    put = put.repeat_interleave(hq // hkv, 1)
+    o = frsa().prompt_attention(q, k, v, bounds([n])).double()
+    assert status() == 0
+    hit = put != 0
+    assert torch.equal(torch.isnan(o[hit]), torch.isnan(put[hit]))
+    same = hit & ~torch.isnan(put)
+    assert torch.equal(o[same], put[same])
+    check(o[~hit], want[0][~hit], want[1][~hit])
+
+
+# ------------------------------------------------------------------ append: sequence boundaries
+def test_append_reports_boundaries_outside_the_tokens():
+    """Sequence boundaries below 0, past the tokens or out of order are reported,
+    wherever they stand; a sequence that begins below 0 is not stored."""
+    g = gen(31)
+    kc, vc, table = paged([48] * 3, 2, 16, 64, BF, g)
+    cosp, sinp = rope_tables(64, 64)
+    q, k, v = (randn(g, 40, h, 64) for h in (4, 2, 2))
+    before = kc.clone(), vc.clone()
+
+    def call(cu):
+        out = frsa().paged_rope_append(q, k, v, kc, vc, table, ints([0, 0, 0]), cosp, sinp,
+                                       cu_seqlens=ints(cu))
+        return out, status()
+
+    (qr, kr), code = call([-3, 40, 40, 40])
+    assert code == 11
+    assert torch.equal(qr, q) and torch.equal(kr, k)
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+    for cu in ([0, 20, 30, 41], [0, 30, 20, 40], [0, -1, 20, 40], [0, 20, 1 << 30, 40]):
+        assert call(cu)[1] == 11, cu
+    for cu in ([0, 20, 30, 40], [5, 5, 30, 38], [40, 40, 40, 40], [0, 0, 0, 0]):
+        assert call(cu)[1] == 0, cu
+    many = [0] * 500 + [40] * 500
+    many[700] = -7
+    table = table[:1].expand(999, -1)
+    out = frsa().paged_rope_append(q, k, v, kc, vc, table, ints([0] * 999), cosp, sinp,
+                                   cu_seqlens=ints(many))
+    assert status() == 11

@@ -145,8 +145,9 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
     bool held = true;
     if (p.cu_seqlens != nullptr) {
       b = find_sequence(p.cu_seqlens, p.B, t, lane);
-      index = t - ld_int(p.cu_seqlens + b);
-      held = index >= 0 && t < ld_int(p.cu_seqlens + b + 1);
+      const int first = ld_int(p.cu_seqlens + b);
+      index = t - first;
+      held = first >= 0 && index >= 0 && t < ld_int(p.cu_seqlens + b + 1);
     }
     index += ld_int(p.start_lens + b);
     const long long pos = !held ? -1 : p.positions != nullptr ? ld_int(p.positions + t) : index;
@@ -171,6 +172,13 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
     if (pos >= 0 && pos < p.n_pos && (lane & 15) < pairs4)
       f = ld_f4((lane < 16 ? p.cosp : p.sinp) + pos * (p.D >> 1) + (lane & 15) * 4);
     turns[warp][lane >> 4][lane & 15] = f;
+  } else if (blockIdx.x == 0 && warp == kAppendMost && p.cu_seqlens != nullptr) {
+    bool bad = false;   // boundaries outside the tokens, or out of order
+    for (int b = lane; b <= p.B; b += 32) {
+      const int c = ld_int(p.cu_seqlens + b);
+      bad |= c < 0 || c > p.T || (b < p.B && ld_int(p.cu_seqlens + b + 1) < c);
+    }
+    if (bad) atomicCAS(&g_dev_status, 0, FRSA_DEV_INDEX);
   }
   __syncthreads();
 
