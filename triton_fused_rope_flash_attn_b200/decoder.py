@@ -13,6 +13,10 @@ per sequence and step:
     with torch.no_grad():
         y = attn.prefill(x, [197, 60], cache)     # x [257, 1024]: the prompts' tokens
         y = attn.step(x_new, cache)               # x_new [2, 1024]: a token each
+
+A sequence that is done gives its pages back (``cache.release(b)``); the others go
+on (``step`` with ``active``), and a new prompt can take its place (``prefill``
+with no tokens for those that run).
 """
 from __future__ import annotations
 
@@ -120,9 +124,12 @@ class CausalRopeAttention(nn.Module):
         return cosp, sinp
 
     def prefill(self, x: torch.Tensor, lens, cache: PagedKVCache) -> torch.Tensor:
-        """Whole prompts, ``x [sum(lens), dim]``, one per sequence of the (empty) cache."""
-        if any(cache.host_lens):
-            raise ValueError("prefill starts from an empty cache")
+        """Whole prompts, ``x [sum(lens), dim]``: ``lens[b]`` tokens for sequence ``b``,
+        which has to be empty; those with no tokens here stay as they are."""
+        for b, (have, n) in enumerate(zip(cache.host_lens, lens)):
+            if have and n:
+                raise ValueError(f"sequence {b} holds {have} tokens: prefill starts from an empty "
+                                 "cache")
         if x.shape[0] != sum(lens):
             raise ValueError(f"{x.shape[0]} tokens for prompts of {sum(lens)}")
         tables = self._tables(lens, cache)
@@ -140,15 +147,29 @@ class CausalRopeAttention(nn.Module):
         o = prompt_attention(q, k, v, cu)
         return self.proj(o.flatten(1))
 
-    def step(self, x: torch.Tensor, cache: PagedKVCache) -> torch.Tensor:
-        """One new token of every sequence, ``x [batch, dim]``."""
-        one = [1] * x.shape[0]
-        tables = self._tables(one, cache)
-        cache.reserve(one)
+    def step(self, x: torch.Tensor, cache: PagedKVCache, active=None) -> torch.Tensor:
+        """One new token of every sequence in ``active`` (a list, in any order; by default
+        all of them), ``x [len(active), dim]``."""
+        batch = len(cache.host_lens)
+        if active is None:
+            new = [1] * x.shape[0]
+        else:
+            active = list(active)
+            if len(set(active)) != len(active) or not all(0 <= b < batch for b in active):
+                raise ValueError(f"active must name sequences of {batch} once each, got {active}")
+            if x.shape[0] != len(active):
+                raise ValueError(f"{x.shape[0]} tokens for {len(active)} sequences")
+            new = [int(b in active) for b in range(batch)]
+        tables = self._tables(new, cache)
+        cache.reserve(new)
         q, k, v = self._project(x)
-        q, _ = paged_rope_append(q, k, v, cache.k, cache.v, cache.block_table, cache.lens,
-                                 *tables,
-                                 positions=cache.lens - 1 if self.has_cls else None)
-        cache.advance(one)
-        o = paged_decode_attention(q, cache.k, cache.v, cache.block_table, cache.lens)
+        table, lens = cache.block_table, cache.lens
+        if active is not None:
+            at = torch.tensor(active, dtype=torch.int64).to(x.device)
+            table, lens = table[at], lens[at]
+        q, _ = paged_rope_append(q, k, v, cache.k, cache.v, table, lens, *tables,
+                                 positions=lens - 1 if self.has_cls else None)
+        cache.advance(new)
+        o = paged_decode_attention(q, cache.k, cache.v, table,
+                                   cache.lens if active is None else lens + 1)
         return self.proj(o.flatten(1))
