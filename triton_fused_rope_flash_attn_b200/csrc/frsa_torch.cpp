@@ -204,15 +204,23 @@ int32_t serve_dtype(const at::Tensor& t) {
   return t.scalar_type() == at::kBFloat16 ? FRSA_DTYPE_BF16 : FRSA_DTYPE_F16;
 }
 
-// A [tokens, heads, D] tensor: on q's device, of q's type, not asking for a gradient.
+// Neither a gradient nor a forward-mode tangent is asked of a tensor.
+void check_no_grad(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+              " requires a gradient: the serving operators have no backward, call them under "
+              "torch.no_grad()");
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name,
+              " has a forward-mode tangent: the serving operators have no derivative");
+}
+
+// A [tokens, heads, D] tensor: on q's device, of q's type, without derivatives.
 void check_tokens(const at::Tensor& t, const at::Tensor& q, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == q.device(), name,
               " must be a CUDA tensor on q's device (there is no CPU path)");
   TORCH_CHECK(t.dim() == 3, name, " must be [tokens, heads, D]");
   TORCH_CHECK_TYPE(t.scalar_type() == q.scalar_type(), name, " must have q's dtype");
   TORCH_CHECK(t.size(2) == q.size(2), name, " must have q's head dim");
-  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()),
-              "the serving operators have no backward: call them under torch.no_grad()");
+  check_no_grad(t, name);
 }
 
 void check_cache(const at::Tensor& c, const at::Tensor& q, const at::Tensor& k_cache,
@@ -227,8 +235,7 @@ void check_cache(const at::Tensor& c, const at::Tensor& q, const at::Tensor& k_c
   TORCH_CHECK(c.stride(3) == 1 && tma_strided_ok(c), name,
               " must have a unit d stride, other strides that are multiples of 16 bytes and "
               "16-byte aligned data");
-  TORCH_CHECK(!(c.requires_grad() && at::GradMode::is_enabled()),
-              "the serving operators have no backward: call them under torch.no_grad()");
+  check_no_grad(c, name);
 }
 
 // An int32 index array on q's device, contiguous.
@@ -313,6 +320,8 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_append(
               "COSP/SINP must be [N_pos, D/2]");
   TORCH_CHECK(cosp.device() == q_in.device() && sinp.device() == q_in.device(),
               "RoPE tables must be on the same device as Q");
+  check_no_grad(cosp, "COSP");
+  check_no_grad(sinp, "SINP");
   const c10::cuda::CUDAGuard guard(q_in.device());
   const int64_t T = q_in.size(0), B = start_lens.numel();
   frsa_paged_append_args a{};
