@@ -51,3 +51,29 @@ def test_tables_that_ask_for_a_gradient_are_refused():
             frsa().paged_rope_append(q, k, v, kc, vc, table, ints([0]), c, s)
         with torch.no_grad():
             frsa().paged_rope_append(q, k, v, kc, vc, table, ints([0]), c, s)
+
+
+def test_append_counts_as_a_write_of_the_caches():
+    """As after an in-place operation of torch: a graph that saved a cache refuses its
+    backward, caches made in inference mode work inside and outside of it."""
+    q, k, v, kc, vc, table, (cosp, sinp) = case()
+    w = torch.ones((), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    for saved in (kc, vc):
+        y = (saved * w).sum()
+        before = kc._version, vc._version
+        frsa().paged_rope_append(q, k, v, kc, vc, table, ints([0]), cosp, sinp)
+        assert kc._version > before[0] and vc._version > before[1]
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    before = kc._version
+    frsa().paged_decode_attention(q, kc, vc, table, ints([1]))
+    assert kc._version == before
+    with torch.inference_mode():
+        kc2, vc2 = kc.clone(), vc.clone()
+        frsa().paged_rope_append(q, k, v, kc2, vc2, table, ints([0]), cosp, sinp)
+        frsa().paged_rope_append(q, k, v, kc, vc, table, ints([0]), cosp, sinp)
+    frsa().paged_rope_append(q, k, v, kc2, vc2, table, ints([0]), cosp, sinp)
+    assert torch.equal(kc, kc2) and torch.equal(vc, vc2)
+    whole = torch.zeros(2, *kc.shape, device="cuda", dtype=torch.bfloat16)   # views share a counter
+    frsa().paged_rope_append(q, k, v, whole[0], whole[1], table, ints([0]), cosp, sinp)
+    assert whole._version > 0

@@ -274,6 +274,12 @@ void lead_strides(int64_t (&dst)[N], const at::Tensor& t) {
   }
 }
 
+// A kernel has written t: as torch's in-place operations do, raise its version
+// (an inference tensor has none).
+void mark_written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // An output of q's type (or `type`) on q's device, without the dispatcher.
 at::Tensor output(at::IntArrayRef sizes, const at::Tensor& q, c10::optional<at::ScalarType> type = {}) {
   return at::detail::empty_cuda(sizes, type.value_or(q.scalar_type()), q.device(), c10::nullopt);
@@ -365,6 +371,10 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_append(
   lead_strides(a.v_strides, v);
   lead_strides(a.cache_strides, k_cache);
   const int rc = g_append(&a, at::cuda::getCurrentCUDAStream().stream());
+  if (rc == FRSA_OK) {
+    mark_written(k_cache);
+    mark_written(v_cache);
+  }
   return {q_out, k_out, rc};
 }
 
