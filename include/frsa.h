@@ -257,7 +257,7 @@ int frsa_convert_out(const frsa_convert_args* args, void* stream);
  * Element strides (token, head) of q, k, v and (page, head, slot) of both
  * caches; the d stride is 1. All zero = contiguous. They are positive
  * multiples of 16 bytes, and the pointers 16-byte aligned. D % 8 == 0,
- * D <= 128; dtype BF16 or F16; scale > 0. */
+ * D <= 128; dtype BF16 or F16; scale > 0, and finite times log2(e). */
 
 /* Append: for token t of sequence b, at index i = start_lens[b] + t -
  * cu_seqlens[b] (cu_seqlens NULL: one token per sequence, T == B), with

@@ -77,3 +77,14 @@ def test_append_counts_as_a_write_of_the_caches():
     whole = torch.zeros(2, *kc.shape, device="cuda", dtype=torch.bfloat16)   # views share a counter
     frsa().paged_rope_append(q, k, v, whole[0], whole[1], table, ints([0]), cosp, sinp)
     assert whole._version > 0
+
+
+@pytest.mark.parametrize("scale", [math.inf, 1e300, 3e38, 1e-60])
+def test_scales_past_their_range_are_refused(scale):
+    q, k, v, kc, vc, table, _ = case()
+    with pytest.raises(ValueError, match="scale"):
+        frsa().paged_decode_attention(q, kc, vc, table, ints([1]), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        frsa().prompt_attention(q, k, v, ints([0, 1]), scale=scale)
+    with pytest.raises(ValueError, match="scale"):   # no call that returns early lets it pass
+        frsa().prompt_attention(q[:0], k[:0], v[:0], ints([0]), scale=scale)

@@ -34,6 +34,9 @@ int serve_cache(int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t
   return FRSA_OK;
 }
 
+// The kernels' exponentials are to the base 2: the scale times log2(e) has to be finite.
+bool scale_ok(float s) { return s > 0.f && s * 1.4426950408889634f <= 3.402823466e38f; }
+
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 // 3-D map {D, heads, T} over packed tokens with (token, head) strides in
@@ -97,7 +100,7 @@ int frsa_paged_decode(const frsa_paged_decode_args* args, void* stream) {
   int rc = serve_common(a.B, a.Hq, a.Hkv, a.D, a.dtype);
   if (rc == FRSA_OK) rc = serve_cache(a.num_pages, a.page_size, a.max_pages, a.block_table_stride);
   if (rc != FRSA_OK) return rc;
-  if (!(a.scale > 0.f)) return FRSA_ERR_BAD_SHAPE;
+  if (!scale_ok(a.scale)) return FRSA_ERR_BAD_SHAPE;
   // The kernel numbers tiles of 64 keys over all (sequence, kv head, head
   // block) units in 31 bits, and page and slot strides in granules in 32.
   const int64_t tiles = (a.max_pages * a.page_size + 63) / 64;
@@ -124,7 +127,7 @@ int frsa_prompt_fwd(const frsa_prompt_args* args, void* stream) {
   int rc = serve_common(a.B, a.Hq, a.Hkv, a.D, a.dtype);
   if (rc != FRSA_OK) return rc;
   const int64_t G = a.Hq / a.Hkv;
-  if (!(a.scale > 0.f) || a.T < 1 || a.T > (int64_t(1) << 30) || G > 128 ||
+  if (!scale_ok(a.scale) || a.T < 1 || a.T > (int64_t(1) << 30) || G > 128 ||
       (a.T / (128 / G) + a.B) * a.Hkv > 0x7FFFFFFFLL)
     return FRSA_ERR_BAD_SHAPE;
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.o) ||

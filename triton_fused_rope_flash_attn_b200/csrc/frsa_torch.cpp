@@ -286,8 +286,11 @@ at::Tensor output(at::IntArrayRef sizes, const at::Tensor& q, c10::optional<at::
 }
 
 float scale_of(const c10::optional<double>& scale, int64_t D) {
-  TORCH_CHECK_VALUE(!scale.has_value() || *scale > 0, "scale must be positive");
-  return static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(double(D)));
+  const float s = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(double(D)));
+  // (the kernels' exponentials are to the base 2)
+  TORCH_CHECK_VALUE(s > 0 && std::isfinite(s * 1.4426950408889634f),
+                    "scale must be positive and finite in float32");
+  return s;
 }
 
 // The split decode's scratch: one per (device, stream), made and zeroed on its
@@ -394,6 +397,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_decode(
   if (with_lse) lse = output({B, q_in.size(1)}, q_in, at::kFloat);
   frsa_paged_decode_args a{};
   a.dtype = serve_dtype(q_in);
+  if (scale.has_value()) a.scale = scale_of(scale, 1);
   if (B == 0 || q_in.size(1) == 0) return {o, lse, 0};
   const at::Tensor q = readable_tokens(q_in);
   const c10::cuda::CUDAStream stream = at::cuda::getCurrentCUDAStream();
@@ -417,7 +421,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> paged_decode(
   a.block_table_stride = bt.size(0) > 1 ? bt.stride(0) : bt.size(1);
   lead_strides(a.q_strides, q);
   lead_strides(a.cache_strides, k_cache);
-  a.scale = scale_of(scale, a.D);
+  if (!scale.has_value()) a.scale = scale_of(scale, a.D);
   const int rc = g_decode(&a, stream.stream());
   return {o, lse, rc};
 }
@@ -439,6 +443,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> prompt(const at::Tensor& q_in, const
   const int64_t T = q_in.size(0), Hq = q_in.size(1);
   frsa_prompt_args a{};
   a.dtype = serve_dtype(q_in);
+  if (scale.has_value()) a.scale = scale_of(scale, 1);
   if (T == 0 || Hq == 0 || cu.size(0) == 1) {   // no sequence: every token belongs to none
     at::Tensor o = at::zeros(q_in.sizes(), q_in.options()), lse;
     if (with_lse) lse = at::full({Hq, T}, -INFINITY, q_in.options().dtype(at::kFloat));
@@ -461,7 +466,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> prompt(const at::Tensor& q_in, const
   lead_strides(a.q_strides, q);
   lead_strides(a.k_strides, k);
   lead_strides(a.v_strides, v);
-  a.scale = scale_of(scale, a.D);
+  if (!scale.has_value()) a.scale = scale_of(scale, a.D);
   const int rc = g_prompt(&a, at::cuda::getCurrentCUDAStream().stream());
   return {o, lse, rc};
 }
