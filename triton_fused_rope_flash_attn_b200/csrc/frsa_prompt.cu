@@ -123,7 +123,7 @@ struct PromptSmem {
   // s_free, pv_done at every key tile: NCH == 1 only (else pv_done at a unit's end).
   uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2];   // p_full: [tile][64-key half]
   uint64_t unit_full[2], unit_empty[2];
-  uint64_t next_full;
+  uint64_t next_full, drained;
   uint64_t mend_full[2], mend_empty[2];
   alignas(16) uint32_t next[4];   // answer to the request for another unit number
   PromptUnit unit[2];
@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(&sm.v_empty[s], 1);
     }
     mbar_init(&sm.next_full, 1);
+    mbar_init(&sm.drained, 1);
     sm.mend_end[0] = sm.mend_end[1] = 0;
     fence_mbar_init();
   }
@@ -640,6 +641,10 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           x = y;
           ++i;
         }
+        // The products complete before the CTA frees the tensor memory and ends,
+        // also where a softmax warp's wait for them gave up.
+        mma_commit_elect(&sm.drained);
+        mbar_wait_limit(&sm.drained, 0);
       }
     }
   } else {
