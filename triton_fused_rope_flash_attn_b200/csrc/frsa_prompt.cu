@@ -53,16 +53,17 @@
 // (478 us, but a row that rises by more than 2^95 within a tile overflows; with a
 // guard against that 486 us and slower on short prompts).
 //
-// Masked places: keys past a row's position get P = 0, but 0 times an
-// infinity or NaN in V (a later token's, or another sequence's in the same
-// tile) would still reach O. It makes NaN, so a row that holds a NaN is looked
-// at again (pr_mend): where NaN in the V of keys that it sees explain it, that
-// is the result; otherwise the row is computed once more in f32, from its keys
-// alone (exact_row). One NaN early in a sequence thus costs the rows behind it a
-// search that ends with the key that holds it. What is computed again are the rows
-// of the tiles at the masked value, and in f16 rows whose P rounds to 0 at an
-// infinity: about 30 instructions a key and row. The limit of the waits applies to
-// the time between two rows then.
+// Masked places: keys past a row's position get P = 0, but 0 times an infinity
+// or NaN in V (a later token's, or another sequence's in the same tile) would
+// still reach O. It makes NaN, so a row that holds a NaN is looked at again
+// (pr_mend): where the V of keys that it sees explains it, by a NaN or infinities
+// of both signs, the NaN stands; by one infinity, that is put in its place;
+// otherwise the row is computed once more in f32, from its keys alone. One NaN in
+// a sequence thus costs the rows behind it a search, which looks first where the
+// last one ended (8192 tokens of 8 and 2 heads of 128: 0.16 ms; with a NaN in the
+// first token's V 0.23, in the middle one's 0.36, with one element of V in a
+// thousand infinite, where most rows see masked ones beside it, 65). The limit of
+// the waits applies to the time between two rows then.
 #include "frsa_internal.h"
 #include "frsa_ptx.cuh"
 #include "frsa_row.cuh"
@@ -296,13 +297,15 @@ struct PrKeys {
   const uint4* v0;
   long long ks, vs;   // token strides in granules
   int n, granules;
+  __device__ int place(int j) const { return j; }
   __device__ const uint4* k(int j) const { return k0 + j * ks; }
   __device__ const uint4* v(int j) const { return v0 + j * vs; }
 };
 
 // The 32 rows from `row0` on of a query tile, as they were written, by a whole warp.
+// `hint`: the token where the last call found a NaN, or -1.
 template <typename T>
-__device__ __forceinline__ void pr_mend(const PromptParams& p, const Mend& a, int row0,
+__device__ __forceinline__ void pr_mend(const PromptParams& p, const Mend& a, int row0, int& hint,
                                         volatile uint32_t* beat) {
   const int lane = threadIdx.x & 31;
   const bool odd = a.odd >> lane & 1;
@@ -320,33 +323,56 @@ __device__ __forceinline__ void pr_mend(const PromptParams& p, const Mend& a, in
     return static_cast<T*>(p.o) + (static_cast<long long>(a.start + token(r)) * p.Hq + head(r)) * p.D;
   };
   if (lane == 0) *beat = *beat + 1;
-  // NaN columns of the lane's row (8 bits a granule) and, at lane & 15 = granule,
-  // of all rows.
-  uint32_t mine[4] = {0u, 0u, 0u, 0u}, want = 0;
-#pragma unroll
-  for (int g = 0; g < 16; ++g) {
-    if (g >= keys.granules) break;
-    const uint32_t bits =
-        odd ? nan_bits<T>(reinterpret_cast<const uint4*>(out(row0 + lane))[g]) : 0u;
-    mine[g >> 2] |= bits << (8 * (g & 3));
-    const uint32_t all = __reduce_or_sync(kWholeWarp, bits);
-    if ((lane & 15) == g) want = all;
-  }
-  // The keys that the first row sees all rows see.
-  const uint32_t seen = __any_sync(kWholeWarp, want != 0)
-                            ? nan_columns<T>(keys, __shfl_sync(kWholeWarp, token(row0) + 1, 0), want)
-                            : 0u;
+  const uint4* mine = reinterpret_cast<const uint4*>(out(row0 + lane));
   bool again = a.redo >> lane & 1;
-#pragma unroll
-  for (int g = 0; g < 16; ++g)
-    again |= (mine[g >> 2] >> (8 * (g & 3)) & 0xffu & ~__shfl_sync(kWholeWarp, seen, g)) != 0;
+  if (a.odd != 0) {
+    // The NaN columns of all rows: 8 bits at lane & 15 = granule.
+    uint32_t want = 0;
+#pragma unroll 1
+    for (int g = 0; g < keys.granules; ++g) {
+      const uint32_t all = __reduce_or_sync(kWholeWarp, odd ? nan_bits<T>(mine[g]) : 0u);
+      if ((lane & 15) == g) want = all;
+    }
+    // What the keys hold that the first row sees, and with it all rows ...
+    const int tok0 = __shfl_sync(kWholeWarp, token(row0), 0), tok = token(row0 + lane);
+    int at = hint - a.start;
+    const uint32_t seen = special_columns<T, 8>(keys, tok0 + 1, want, at);
+    hint = a.start + at;
+    if (__any_sync(kWholeWarp, (want & ~explained(seen)) != 0)) {
+      // ... and those up to the row itself (fewer than 32; lane i looks at K of the
+      // i-th of them).
+      const int more = token(row0 + 31 - __clz(a.odd)) - tok0;
+      uint32_t k_odd = 0;
+      if (lane < more)
+#pragma unroll 1
+        for (int g = 0; g < keys.granules; ++g)
+          k_odd |= bits_from(keys.k(tok0 + 1 + lane)[g], kInf<T>);
+      const unsigned unsure = __ballot_sync(kWholeWarp, k_odd != 0);
+#pragma unroll 1
+      for (int g = 0; g < keys.granules; ++g) {
+        const uint32_t nan = odd ? nan_bits<T>(mine[g]) : 0u;
+        uint32_t holds = __shfl_sync(kWholeWarp, seen, g);
+        if (!__any_sync(kWholeWarp, (nan & ~explained(holds)) != 0)) continue;
+#pragma unroll 1
+        for (int i = 0; i < more; ++i) {
+          uint32_t x = special_bits<T>(keys.v(tok0 + 1 + i)[g]);
+          if (unsure >> i & 1) x = (x & 0xffu) | ((x >> 8 | x >> 16) & 0xffu) << 24;
+          if (tok0 + 1 + i <= tok) holds |= x;
+        }
+        const Mended m = explain(nan, holds);
+        again |= m.left != 0;
+        put_infinities(out(row0 + lane) + g * 8, m);
+      }
+    }
+    __syncwarp();
+  }
   unsigned todo = __ballot_sync(kWholeWarp, again);
   while (todo != 0) {
     const int i = __ffs(todo) - 1, r = row0 + i;
     todo &= todo - 1;
     if (lane == 0) *beat = *beat + 1;
     keys.n = __shfl_sync(kWholeWarp, token(r) + 1, 0);
-    const float lse = exact_row<T>(
+    const float lse = exact_row<T, 4>(
         keys, static_cast<const T*>(p.q) + (a.start + token(r)) * p.qs[0] + head(r) * p.qs[1],
         p.c2, out(r));
     if (p.lse != nullptr && lane == i)
@@ -528,6 +554,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       }
     } else if (warp == 3) {
       // ------------------------------------------------------------ mender
+      int hint = -1;
       for (int i = 0;; ++i) {
         const int s = i & 1;
         if (!__all_sync(kWholeWarp, wait(&sm.mend_full[s], (i >> 1) & 1))) break;
@@ -536,7 +563,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         for (int w = 0; w < 8; ++w) {
           const Mend a = sm.mend[s][w];
           if ((a.odd | a.redo) != 0)
-            pr_mend<T>(p, a, (w & 3) * 32, &sm.beat);
+            pr_mend<T>(p, a, (w & 3) * 32, hint, &sm.beat);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.mend_empty[s]);
