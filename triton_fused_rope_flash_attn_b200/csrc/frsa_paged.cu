@@ -251,17 +251,18 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const A
 // does not depend on who comes last.
 //
 // What bounds it: memory. SMs do not read at the same speed: of 296 equal
-// shares of one 131072-token sequence (8 kv heads, 537 MB) the first is done
-// after 64 us, half after 78 and the last after 97. Tried against that and not
+// shares of one 131072-token sequence (8 kv heads, 537 MB) the first has computed
+// its tiles after 67 to 71 us, half after 78 and the last after 83 to 87; the last
+// join ends at 91 to 95 (time stamps in three launches). Tried against that and not
 // faster: further, smaller shares claimed from a ticket counter (all done
 // between 80 and 94 us, but with four times the partials, whose joining took
 // the gain back, in the kernel or in a second one); a fifth warp that copies
 // for all four (a 16-row TMA box takes about 100 cycles: 122 us in all for
 // pages of 16, though 177 against 187 for 64 sequences with pages of 64) or
-// that only schedules. Now 97 us of a call for 131072 tokens (5.5 TB/s), 176 for
-// 64 sequences of up to 8000 tokens (5.9 TB/s, 91 % of the measured copy rate);
-// of 6.0 us for 197 tokens, 2 pass before the first copies (lengths, pages),
-// 1 until they land, 1.5 over four tiles.
+// that only schedules. Now 98 us of a call for 131072 tokens (5.5 TB/s), 178 for
+// 64 sequences of up to 8000 tokens (5.8 TB/s, 90 % of the measured copy rate);
+// of 5.9 us for 197 tokens, 2.1 pass before the first copies (lengths, pages), the
+// four tiles are computed after 4.3, the row is written after 4.8.
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16;                        // keys of a warp in a tile
@@ -1058,7 +1059,9 @@ cudaError_t launch_decode_nk(DecodeParams& p, int grid, cudaStream_t stream) {
   return launch_decode_t<T, 8, NT>(p, grid, stream);
 }
 
-// Groups of up to 8 query heads take 8 columns, larger ones blocks of 16.
+// Groups of up to 8 query heads take 8 columns, larger ones blocks of 16, each of
+// which reads the keys again, mostly from L2 (4 sequences of 16384 tokens, 2 kv
+// heads of 128: groups of 8 take 22 us, of 16 32, of 17 36, of 32 37, of 64 54).
 template <typename T>
 cudaError_t launch_decode_heads(DecodeParams& p, int grid, cudaStream_t stream) {
   const int heads = p.group <= 8 ? 8 : 16;

@@ -13,11 +13,12 @@
 //
 //   warp 0       TMA producer: the unit's query tiles, then K and V tiles of
 //                128 keys into rings of KS stages
-//   warp 1       TMEM allocator + single-thread tcgen05.mma issuer: P V and the
-//                next scores of one query tile, then of the other, so that one
-//                is in its softmax while the other's products run (with a
-//                thread per query tile both came into step: 673 against 637 us
-//                for one prompt of 8192 tokens)
+//   warp 1       TMEM allocator + tcgen05.mma issuer (the whole warp runs it, one
+//                elected lane issues): P V and the next scores of one query tile,
+//                then of the other, so that one is in its softmax while the
+//                other's products run (with an issuer per query tile both came
+//                into step: 673 against 637 us for one prompt of 8192 tokens, in
+//                an earlier state)
 //   warp 2       scheduler: turns unit numbers into units, one ahead. The grid
 //                has one CTA per unit number; a running CTA takes over the
 //                next one that has not started (clusterlaunchcontrol), so the
@@ -34,24 +35,25 @@
 // columns from 256 g + 128 on for O, which accumulates there over the unit's
 // key tiles. P is written as packed 16-bit pairs: for D <= 64 into columns of
 // its own (256 g + 192 on), so that the next scores are computed as soon as
-// these have been read; for larger D over the scores, since TMEM is full. The
+// these have been read; for larger D over the scores: with key tiles of 128, P
+// takes 64 columns and O leaves 128 - D of them. The
 // softmax base is raised (and O rescaled) only when a tile's maximum leaves
 // the range above it (PrBase). P of a tile's first 64 keys is published before the
 // rest is computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
 //
-// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 491
-// us, 1120 TFLOP/s, 67 % of the card's measured rate (more over longer runs,
-// when the card lowers its clocks under the power limit). Per 128 keys of a query
-// tile 1.5 us of softmax (0.3 of them waits for TMEM, the rest about 600
-// instructions on a chain per row) and 0.4 us of products before the next
-// scores; the two tiles share the SM's exponentials and its tensor core, of
-// each of which they use 61 %. Tried and not faster: two threads per row; a
+// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 503
+// us over repeated calls, 1093 TFLOP/s, 66 % of the card's measured rate (479
+// in a single one, before the card lowers its clocks under the power limit). Per
+// 128 keys of a query tile 1.5 us of softmax (0.3 of them waits for TMEM, the
+// rest about 600 instructions on a chain per row) and 0.4 us of products before
+// the next scores; the two tiles share the SM's exponentials and its tensor core,
+// of each of which they use 60 %. Tried and not faster: two threads per row; a
 // fourth or an eighth of the exponentials by a polynomial on the FMA pipe; a
 // thread of its own for each tile's products. Not kept: for bf16, whose range
 // would allow it, no maximum per tile but a base raised when the sum has grown
-// (478 us, but a row that rises by more than 2^95 within a tile overflows; with a
-// guard against that 486 us and slower on short prompts).
+// (478 against then 491 us, but a row that rises by more than 2^95 within a tile
+// overflows; with a guard against that 486 us and slower on short prompts).
 //
 // Masked places: keys past a row's position get P = 0, but 0 times an infinity
 // or NaN in V (a later token's, or another sequence's in the same tile) would
@@ -165,8 +167,12 @@ __device__ __forceinline__ int pr_units_of(const PromptParams& p, int b) {
 
 // Unit number -> unit, by a whole warp. Up to 32 sequences the longest units
 // come first over all sequences (a unit of query block t reads about t key
-// blocks, so: by descending t); beyond that, sequence after sequence, each
-// with its longest units first.
+// blocks, so: by descending t); beyond that, where a lane would hold several
+// sequences, sequence after sequence, each with its longest units first. What the
+// order is worth (32 and 8 heads of 128): one of 2048 tokens before 40 of 64 takes
+// 53 us, behind them 62; before or behind 31 of them, 53. The search reads about
+// B / 32 pairs of boundaries for each unit, so many tiny sequences cost more than
+// their work: 1000 of 16 tokens 0.59 ms, 2000 of them 2.1.
 __device__ __forceinline__ PromptUnit pr_find_unit(const PromptParams& p, int id, int lane) {
   PromptUnit x;
   x.valid = 0;

@@ -17,7 +17,9 @@ place, others are copied; the caches are used in place and must be so
 addressable. Everything runs on torch's current stream, without a host
 synchronisation. Index values outside their range (a page, a position, a
 length) are not followed; ``frsa_query_status`` of the C ABI reports them.
-There is no backward: inputs that ask for a gradient are refused.
+There is no derivative: inputs that ask for a gradient, or carry a forward-mode
+tangent, are refused. What is not finite in a token's keys and values counts as
+in the formula for those that see it, and not at all for others.
 """
 from __future__ import annotations
 
@@ -38,7 +40,7 @@ def paged_rope_append(q, k, v, k_cache, v_cache, block_table, start_lens, cosp, 
     ``positions[t]`` (``[T]``; -1: not rotated, as a CLS token) where given.
 
     Returns the rotated ``(q, k)``, contiguous, rounded once; ``k_cache`` and
-    ``v_cache`` are written in place. Tokens outside ``[cu_seqlens[0],
+    ``v_cache`` are written in place (their version counters rise). Tokens outside ``[cu_seqlens[0],
     cu_seqlens[-1])`` belong to no sequence: neither rotated nor stored.
     """
     q_out, k_out, rc = _ext().paged_append(q, k, v, k_cache, v_cache, block_table, start_lens,
@@ -53,7 +55,8 @@ def paged_decode_attention(q, k_cache, v_cache, block_table, seq_lens, scale=Non
     """Attention of one (rotated) query token per sequence over its cached tokens.
 
     ``q [B, Hq, D]``, ``seq_lens [B]``: cached tokens, the new one included
-    (0: the output is 0 and the LSE -inf). ``scale`` defaults to ``1/sqrt(D)``.
+    (0: the output is 0 and the LSE -inf). ``scale`` (positive, finite) defaults
+    to ``1/sqrt(D)``.
     Returns ``o [B, Hq, D]``, with ``return_lse`` also the natural-log row LSE
     (float32 ``[B, Hq]``). The split over the cache's length is joined in a
     fixed order: equal inputs give equal bits.
