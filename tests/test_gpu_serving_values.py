@@ -414,3 +414,36 @@ def test_append_reports_boundaries_outside_the_tokens():
     out = frsa().paged_rope_append(q, k, v, kc, vc, table, ints([0] * 999), cosp, sinp,
                                    cu_seqlens=ints(many))
     assert status() == 11
+
+
+@pytest.mark.parametrize("which", ["prompt", "decode"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_infinity_of_no_weight_in_a_row_computed_again(which, dtype):
+    """An infinity 200 nats below the largest score (zero in 32 bits) in a row that is
+    computed again for another column: a key of -inf score whose v is infinite (0
+    times an infinity: NaN) in the decode, a masked value in the prompt."""
+    n, D = 300, 64
+    g = gen(77)
+    q, k = (torch.zeros(n, 1, D, device="cuda", dtype=dtype) for _ in range(2))
+    q[..., 0] = 1.0
+    k[0, 0, 0] = 200.0
+    v = randn(g, n, 1, D, dtype=dtype)
+    v[100, 0, 9] = math.inf
+    if which == "prompt":
+        v[250, 0, 20] = math.nan   # masked for rows 192..249 of its tile
+        o = frsa().prompt_attention(q, k, v, bounds([n]), scale=1.0)[192:250, 0]
+        bad = []
+    else:
+        k[150, 0, 0] = -math.inf
+        v[150, 0, 20] = math.inf
+        kc, vc, table = paged([n], 1, 16, D, dtype, g)
+        at = torch.arange(n, device="cuda")
+        kc[table[0, at // 16].long(), :, at % 16] = k
+        vc[table[0, at // 16].long(), :, at % 16] = v
+        o = frsa().paged_decode_attention(q[:1], kc, vc, table, ints([n]), scale=1.0)[0]
+        bad = [20]
+    assert status() == 0
+    assert (o[:, 9] == math.inf).all()
+    rest = [c for c in range(D) if c != 9 and c not in bad]
+    assert torch.equal(o[:, rest], v[0, 0, rest].expand(o.shape[0], -1))
+    assert torch.isnan(o[:, bad]).all()

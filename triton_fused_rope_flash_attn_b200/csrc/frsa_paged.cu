@@ -472,9 +472,16 @@ __device__ __noinline__ void dec_mend(const DecKeys& keys, const T* q, float c2,
   if (g < keys.granules) want = nan_bits<T>(reinterpret_cast<const uint4*>(orow)[g]);
   if (!__any_sync(kWholeWarp, want != 0)) return;
   int hint = -1;
-  const Mended m = explain(want, special_columns<T, 4>(keys, keys.n, want, hint));
-  if (__any_sync(kWholeWarp, m.left != 0)) exact_row<T, 2>(keys, q, c2, orow);
-  else if (lane < 16) put_infinities(orow + g * 8, m);
+  const uint32_t seen = special_columns<T, 4>(keys, keys.n, want, hint);
+  Mended m = explain(want, seen);
+  if (__any_sync(kWholeWarp, m.left != 0)) {
+    exact_row<T, 2>(keys, q, c2, orow);
+    __syncwarp();
+    // (an infinity whose weight is 0 in f32 makes NaN there too)
+    if (g < keys.granules) m = explain(nan_bits<T>(reinterpret_cast<const uint4*>(orow)[g]), seen);
+    __syncwarp();
+  }
+  if (lane < 16) put_infinities(orow + g * 8, m);
 }
 
 template <typename T, int NK, int NT>

@@ -330,21 +330,25 @@ __device__ __forceinline__ void pr_mend(const PromptParams& p, const Mend& a, in
   };
   if (lane == 0) *beat = *beat + 1;
   const uint4* mine = reinterpret_cast<const uint4*>(out(row0 + lane));
-  bool again = a.redo >> lane & 1;
+  const int tok0 = __shfl_sync(kWholeWarp, token(row0), 0), tok = token(row0 + lane);
+  uint32_t want = 0, seen = 0;   // 8 columns at lane & 15 = granule
   if (a.odd != 0) {
-    // The NaN columns of all rows: 8 bits at lane & 15 = granule.
-    uint32_t want = 0;
+    // The NaN columns of all rows, and what the keys hold there that the first row
+    // sees, and with it all rows ...
 #pragma unroll 1
     for (int g = 0; g < keys.granules; ++g) {
       const uint32_t all = __reduce_or_sync(kWholeWarp, odd ? nan_bits<T>(mine[g]) : 0u);
       if ((lane & 15) == g) want = all;
     }
-    // What the keys hold that the first row sees, and with it all rows ...
-    const int tok0 = __shfl_sync(kWholeWarp, token(row0), 0), tok = token(row0 + lane);
     int at = hint - a.start;
-    const uint32_t seen = special_columns<T, 8>(keys, tok0 + 1, want, at);
+    seen = special_columns<T, 8>(keys, tok0 + 1, want, at);
     hint = a.start + at;
-    if (__any_sync(kWholeWarp, (want & ~explained(seen)) != 0)) {
+  }
+  bool again = a.redo >> lane & 1;
+  const bool search = __any_sync(kWholeWarp, (want & ~explained(seen)) != 0);
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    if (search) {
       // ... and those up to the row itself (fewer than 32; lane i looks at K of the
       // i-th of them).
       const int more = token(row0 + 31 - __clz(a.odd)) - tok0;
@@ -369,20 +373,25 @@ __device__ __forceinline__ void pr_mend(const PromptParams& p, const Mend& a, in
         again |= m.left != 0;
         put_infinities(out(row0 + lane) + g * 8, m);
       }
+      __syncwarp();
+    }
+    // (The second time only for rows that were computed again: an infinity whose
+    // weight is 0 in f32 makes NaN there too.)
+    if (pass == 1) break;
+    unsigned todo = __ballot_sync(kWholeWarp, again);
+    if (todo == 0) break;
+    while (todo != 0) {
+      const int i = __ffs(todo) - 1, r = row0 + i;
+      todo &= todo - 1;
+      if (lane == 0) *beat = *beat + 1;
+      keys.n = __shfl_sync(kWholeWarp, token(r) + 1, 0);
+      const float lse = exact_row<T, 4>(
+          keys, static_cast<const T*>(p.q) + (a.start + token(r)) * p.qs[0] + head(r) * p.qs[1],
+          p.c2, out(r));
+      if (p.lse != nullptr && lane == i)
+        p.lse[static_cast<long long>(head(r)) * p.T + a.start + token(r)] = lse;
     }
     __syncwarp();
-  }
-  unsigned todo = __ballot_sync(kWholeWarp, again);
-  while (todo != 0) {
-    const int i = __ffs(todo) - 1, r = row0 + i;
-    todo &= todo - 1;
-    if (lane == 0) *beat = *beat + 1;
-    keys.n = __shfl_sync(kWholeWarp, token(r) + 1, 0);
-    const float lse = exact_row<T, 4>(
-        keys, static_cast<const T*>(p.q) + (a.start + token(r)) * p.qs[0] + head(r) * p.qs[1],
-        p.c2, out(r));
-    if (p.lse != nullptr && lane == i)
-      p.lse[static_cast<long long>(head(r)) * p.T + a.start + token(r)] = lse;
   }
 }
 
