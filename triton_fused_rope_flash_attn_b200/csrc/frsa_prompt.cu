@@ -42,8 +42,8 @@
 // rest is computed. The products of a tile's last keys are cut to the 16-key steps
 // that some row can see.
 //
-// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 503
-// us over repeated calls, 1093 TFLOP/s, 66 % of the card's measured rate (479
+// What bounds it: for one prompt of 8192 tokens (32 and 8 heads, D = 128) 509
+// us over repeated calls, 1080 TFLOP/s, 65 % of the card's measured rate (479
 // in a single one, before the card lowers its clocks under the power limit). Per
 // 128 keys of a query tile 1.5 us of softmax (0.3 of them waits for TMEM, the
 // rest about 600 instructions on a chain per row) and 0.4 us of products before
